@@ -13,12 +13,12 @@ from .all_reduce import _all_reduce
 from .ext import reduce_scatter_mpi, all_gather_mpi
 from .request import Request, StreamRequest
 from .virtual import VirtualWorld, VirtualComm, VirtualRankError
-from . import kernels, build_kernels
+from . import kernels, build_kernels, optim
 
 __all__ = [
     "ProcessGroups", "all_gather_2D", "_all_gather", "recursive_doubling_allgather_mpi",
     "reduce_scatter_2D", "_reduce_scatter", "recursive_halving_reduce_scatter_mpi",
     "ring_reduce_scatter_mpi", "_all_reduce", "reduce_scatter_mpi", "all_gather_mpi",
     "Request", "StreamRequest", "VirtualWorld", "VirtualComm", "VirtualRankError",
-    "kernels", "build_kernels",
+    "kernels", "build_kernels", "optim",
 ]
