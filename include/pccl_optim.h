@@ -83,7 +83,7 @@ int pccl_optim_plan_adamw8(pccl_optim_plan** plan, void* const* params, const vo
                            const int* copy_dtype, int count);
 
 typedef struct {
-  double lr, beta1, beta2, eps, weight_decay;
+  double lr, beta1, beta2, eps, weight_decay;   /* eps: 0, or a normal fp32 number */
   double grad_scale;        /* factor of every gradient, e.g. 1 / (loss scale * ranks); not 0 */
   double max_norm;          /* clip to this norm; 0 = no clipping */
   int64_t step;             /* t, 1 for the first step */
@@ -95,10 +95,23 @@ typedef struct {
   uint32_t seed;            /* of the stochastic rounding; the random bits depend on seed, step and element index */
 } pccl_optim_step;
 
+/* The addresses of a plan's tensors travel in kernel arguments, which hold 64
+ * (AdamW) or 56 (8-bit) tensors of the same types a launch.  For a plan with
+ * more, pccl_optim_table_bytes says how large a table of all of them is (0:
+ * there is nothing to gain); pccl_optim_table_fill writes it into HOST memory,
+ * and the caller copies it to the GPU, to a multiple of 64 bytes.  A run that is
+ * given that copy takes one launch per 4096 tensors.  The copy has to be
+ * complete before the run on its stream and to stay until the run is done; a
+ * captured run reads it at every replay. */
+size_t pccl_optim_table_bytes(const pccl_optim_plan* plan);
+int pccl_optim_table_fill(const pccl_optim_plan* plan, void* host, size_t bytes);
+
 /* One step.  grads: NULL for the gradients of the plan, or others of the same
  * lengths and types (a table of `count` pointers) that share no memory with
- * what the plan writes. */
-int pccl_optim_run_adamw(const pccl_optim_plan* plan, const void* const* grads, const pccl_optim_step* step, void* stream);
+ * what the plan writes.  table: NULL, or the plan's table in device memory
+ * (ignored with other gradients, whose addresses it does not have). */
+int pccl_optim_run_adamw(const pccl_optim_plan* plan, const void* const* grads, const void* table,
+                         const pccl_optim_step* step, void* stream);
 
 /* ---- gradient norm -------------------------------------------------------
  * out[0] = sqrt(sum of x^2 over all elements of all tensors), fp32; 0 for no

@@ -60,8 +60,12 @@ constexpr size_t kStreamFrom = (size_t)288 << 20;
 // Work items of one launch.  The grid is counted in threads, in 32 bits.
 constexpr size_t kMaxItems = ((size_t)1 << 26) - 1;
 
-constexpr int kAdamUnroll = 1;        // blocks of 256 elements per wave of k_adamw
-constexpr uint32_t kNormGroups = 1024;    // workgroups (and partial sums) of one launch of the norm
+// Work of one wave (see the kernels): blocks of 256 elements for k_quantize, by the size of the source's element, and
+// for k_dequantize
+constexpr int kQuantizeWide = 4, kQuantizeNarrow = 8, kDequantizeBlocks = 4;
+
+constexpr int kNormThreads = 1024;        // threads of a workgroup of the norm
+constexpr uint32_t kNormGroups = 256;     // workgroups, and partial sums, of one launch
 
 size_t esize_of(int dtype) {
   return dtype == PCCL_HIP_F32 ? 4 : (dtype == PCCL_HIP_BF16 || dtype == PCCL_HIP_F16) ? 2 : 0;
@@ -69,7 +73,7 @@ size_t esize_of(int dtype) {
 
 enum Kind { kAdamW, kAdamW8, kNorm, kQuantize, kDequantize };
 
-// The tensors of one launch: alike in their types, at most as many as its table holds
+// Tensors that are alike in their types, for one launch or a few
 struct Batch {
   int p, g, c;                 // element types; c = PCCL_OPTIM_NONE without a copy
   std::vector<int> tensor;     // their places in the plan
@@ -153,20 +157,21 @@ int check_apart(const pccl_optim_plan& plan, const void* p, size_t bytes, const 
   return PCCL_HIP_OK;
 }
 
-// Puts the tensors that are not empty into launches: alike in type, in their order.
-int make_batches(pccl_optim_plan& plan, const int* p, const int* g, const int* c, size_t per_item, int cap, const char* what) {
+// Puts the tensors that are not empty into batches: alike in type, in their
+// order, at most `cap` of them.  items_of(i): the work items of tensor i.
+template <class F>
+int make_batches(pccl_optim_plan& plan, const int* p, const int* g, const int* c, F&& items_of, size_t cap, const char* what) {
   for (int i = 0; i < plan.count; ++i) {
-    const size_t n = plan.n[i];
-    if (!n) continue;
-    const int pt = p ? p[i] : 0, gt = g ? g[i] : 0, ct = c ? c[i] : PCCL_OPTIM_NONE;
-    const size_t items = (n + per_item - 1) / per_item;
-    if (n > PCCL_OPTIM_MAX_ELEMENTS || items > kMaxItems)
-      return fail(PCCL_HIP_EINVAL, "%s: tensor %d has %zu elements, more than %zu", what, i, n, (size_t)PCCL_OPTIM_MAX_ELEMENTS);
+    if (!plan.n[i]) continue;
+    const int pt = p[i], gt = g ? g[i] : 0, ct = c ? c[i] : PCCL_OPTIM_NONE;
+    const size_t items = items_of(i);
+    if (items > kMaxItems)
+      return fail(PCCL_HIP_EINVAL, "%s: tensor %d has %zu elements, more than one launch takes", what, i, plan.n[i]);
     Batch* to = nullptr;
-    for (auto b = plan.batches.rbegin(); b != plan.batches.rend() && !to; ++b)
-      if (b->p == pt && b->g == gt && b->c == ct) {
-        if ((int)b->tensor.size() < cap && b->items + items <= kMaxItems) to = &*b;
-        else break;      // only the last batch of these types is open
+    for (auto b = plan.batches.rbegin(); b != plan.batches.rend(); ++b)
+      if (b->p == pt && b->g == gt && b->c == ct) {     // the last one of these types is the one that is open
+        if (b->tensor.size() < cap && b->items + items <= kMaxItems) to = &*b;
+        break;
       }
     if (!to) {
       plan.batches.push_back(Batch{pt, gt, ct, {}, {}, 0});
@@ -177,6 +182,73 @@ int make_batches(pccl_optim_plan& plan, const int* p, const int* g, const int* c
     to->items += (uint32_t)items;
   }
   return PCCL_HIP_OK;
+}
+
+// The entries of tensors in a table
+void fill(AdamEntry& e, const pccl_optim_plan& plan, int i, const void* const* grads) {
+  e = AdamEntry{plan.a[i], grads ? grads[i] : plan.g[i], plan.b[i], plan.c[i], plan.d[i], plan.n[i]};
+}
+void fill(Adam8Entry& e, const pccl_optim_plan& plan, int i, const void* const* grads) {
+  e = Adam8Entry{plan.a[i], grads ? grads[i] : plan.g[i], plan.b[i], plan.c[i], (float*)plan.e[i], (float*)plan.f[i],
+                 plan.d[i], plan.n[i]};
+}
+void fill(BlocksEntry& e, const pccl_optim_plan& plan, int i, const void* const*) {
+  e = BlocksEntry{plan.a[i], (float*)plan.b[i], plan.c[i], plan.n[i]};
+}
+void fill(NormEntry& e, const pccl_optim_plan& plan, int i, const void* const*) { e = NormEntry{plan.g[i], plan.n[i]}; }
+
+// A launch's share of a batch
+struct Share {
+  int count;
+  uint32_t items;
+  const void* dev;     // the table in device memory, or NULL
+};
+
+// launch(table, share) for a batch: once where its table lies in device memory,
+// else as often as it takes to pass all tensors in kernel arguments.
+template <class T, class F>
+void each_launch(const pccl_optim_plan& plan, const Batch& b, const void* const* grads, const void* dev, F&& launch) {
+  T t;
+  const int total = (int)b.tensor.size();
+  if (dev) {
+    launch(t, Share{total, b.items, dev});
+    return;
+  }
+  for (int k0 = 0; k0 < total; k0 += T::kInline) {
+    const int count = std::min(total - k0, T::kInline);
+    for (int k = 0; k < count; ++k) {
+      fill(t.e[k], plan, b.tensor[k0 + k], grads);
+      t.start[k] = b.start[k0 + k] - b.start[k0];
+    }
+    const uint32_t end = k0 + count < total ? b.start[k0 + count] : b.items;
+    launch(t, Share{count, end - b.start[k0], nullptr});
+  }
+}
+
+// Device tables: batch after batch, each its entries and then their first work items, from multiples of 64 bytes
+template <class E> size_t table_size(const Batch& b) {
+  return (b.tensor.size() * (sizeof(E) + sizeof(uint32_t)) + 63) / 64 * 64;
+}
+template <class T> size_t table_bytes(const pccl_optim_plan& plan) {
+  size_t bytes = 0;
+  bool more = false;         // than one launch takes in its arguments: only then is a table worth having
+  for (const Batch& b : plan.batches) {
+    bytes += table_size<typename T::entry>(b);
+    more = more || b.tensor.size() > (size_t)T::kInline;
+  }
+  return more ? bytes : 0;
+}
+template <class T> void table_fill(const pccl_optim_plan& plan, char* to) {
+  typedef typename T::entry E;
+  for (const Batch& b : plan.batches) {
+    for (size_t k = 0; k < b.tensor.size(); ++k) {
+      E e;
+      fill(e, plan, b.tensor[k], nullptr);
+      memcpy(to + k * sizeof(E), &e, sizeof(E));
+      memcpy(to + b.tensor.size() * sizeof(E) + k * sizeof(uint32_t), &b.start[k], sizeof(uint32_t));
+    }
+    to += table_size<E>(b);
+  }
 }
 
 // Runs `make` on a new plan.  Nothing that the standard library throws leaves the library.
@@ -193,13 +265,12 @@ int new_plan(pccl_optim_plan** out, Kind kind, int count, const size_t* n, const
     plan->kind = kind;
     plan->count = count;
     plan->n.assign(n, n + count);
-    for (int i = 0; i < count; ++i)
-      if (n[i] > PCCL_OPTIM_MAX_ELEMENTS) {
-        delete plan;
-        return fail(PCCL_HIP_EINVAL, "%s: tensor %d has %zu elements, more than %zu", what, i, n[i], (size_t)PCCL_OPTIM_MAX_ELEMENTS);
-      }
     Checker check{*plan, what, {}};
-    rc = make(*plan, check);
+    rc = PCCL_HIP_OK;
+    for (int i = 0; i < count && !rc; ++i)
+      if (n[i] > PCCL_OPTIM_MAX_ELEMENTS)
+        rc = fail(PCCL_HIP_EINVAL, "%s: tensor %d has %zu elements, more than %zu", what, i, n[i], (size_t)PCCL_OPTIM_MAX_ELEMENTS);
+    if (!rc) rc = make(*plan, check);
     if (!rc) {
       rc = check.overlaps();
       size_t bytes = 0;
@@ -214,12 +285,13 @@ int new_plan(pccl_optim_plan** out, Kind kind, int count, const size_t* n, const
   return PCCL_HIP_OK;
 }
 
+size_t items_for(size_t n, size_t per) { return (n + per - 1) / per; }
 size_t blocks_of(size_t n) { return (n + kBlock - 1) / kBlock; }
 
 // What AdamW with moments of either width checks and keeps.
 int make_adamw(pccl_optim_plan& plan, Checker& check, void* const* params, const void* const* grads, void* const* m,
                void* const* v, float* const* ms, float* const* vs, void* const* copies, const int* pt, const int* gt,
-               const int* ct, size_t per_item, int cap) {
+               const int* ct) {
   const bool eight = plan.kind == kAdamW8;
   const char* vname = eight ? "exp_avg_rms" : "exp_avg_sq";
   int rc;
@@ -256,7 +328,8 @@ int make_adamw(pccl_optim_plan& plan, Checker& check, void* const* params, const
     plan.f.push_back(eight ? vs[i] : nullptr);
     plan.gtype.push_back(gt[i]);
   }
-  return make_batches(plan, pt, gt, ctype.data(), per_item, cap, check.what);
+  return make_batches(plan, pt, gt, ctype.data(), [&](int i) { return blocks_of(plan.n[i] + (eight ? 0 : lead(m[i]))); },
+                      kTableMax, check.what);
 }
 
 int make_hyper(const pccl_optim_plan& plan, const pccl_optim_step& s, Hyper& h, const char* what) {
@@ -264,7 +337,7 @@ int make_hyper(const pccl_optim_plan& plan, const pccl_optim_step& s, Hyper& h, 
   if (!(s.lr >= 0) || !std::isfinite(s.lr)) return bad("lr", s.lr);
   if (!(s.beta1 >= 0 && s.beta1 < 1)) return bad("beta1", s.beta1);
   if (!(s.beta2 >= 0 && s.beta2 < 1)) return bad("beta2", s.beta2);
-  if (!(s.eps >= 0) || !std::isfinite(s.eps)) return bad("eps", s.eps);
+  if (!(s.eps >= 0) || !std::isfinite(s.eps) || (s.eps > 0 && s.eps < 0x1p-126)) return bad("eps", s.eps);
   if (!(s.weight_decay >= 0) || !std::isfinite(s.weight_decay)) return bad("weight_decay", s.weight_decay);
   if (!std::isfinite(s.grad_scale) || (float)s.grad_scale == 0.0f || std::isinf((float)s.grad_scale)) return bad("grad_scale", s.grad_scale);
   if (!(s.max_norm >= 0) || !std::isfinite(s.max_norm)) return bad("max_norm", s.max_norm);
@@ -322,29 +395,38 @@ template <class F> void with_types(const Batch& b, F&& f) {
   else with_grad<F16>(b.g, b.c, f);
 }
 
-struct AdamLaunch {
-  const AdamTable& t;
-  const Batch& b;
-  const Hyper& h;
-  bool nt;
-  hipStream_t stream;
-  template <class P, class G, class C> void operator()() const {
-    const int count = (int)b.tensor.size();
-    if (nt) PCCL_LAUNCH((k_adamw<P, G, C, kAdamUnroll, true>), dim3(b.items), dim3(kWave), 0, stream, t, count, h);
-    else PCCL_LAUNCH((k_adamw<P, G, C, kAdamUnroll, false>), dim3(b.items), dim3(kWave), 0, stream, t, count, h);
-  }
-};
+// Unused LDS of a workgroup of k_adamw when it streams from HBM: it takes the
+// room of further waves on a CU (160 KiB of LDS), and fewer of them ask the
+// memory for a narrower window of each of the 7-9 streams at any moment.
+// Measured on MI355X, 8 tensors of 32 Mi elements, us at 0 / 6 / 8 / 9 / 10 / 11 / 13 KiB:
+//   fp32 parameters, bf16 gradients, bf16 copy   1264 1244 1193 1179 1181 1167 1180
+//   fp32 parameters, fp32 gradients              1219 1227 1183 1164 1163 1150 1144
+//   bf16 parameters, bf16 gradients               942  923  905  905  905  914  969
+// k_adamw8, which computes more per byte, loses by every limit that has an
+// effect (688 without, 737 at 6 KiB).
+unsigned adamw_lds(const pccl_optim_plan& plan, const Batch& b) {
+  return !plan.stream ? 0 : b.p == PCCL_HIP_F32 ? 11264 : 8192;
+}
 
-struct Adam8Launch {
-  const Adam8Table& t;
+struct AdamLaunch {
+  const pccl_optim_plan& plan;
   const Batch& b;
   const Hyper& h;
-  bool nt;
+  const void* const* grads;
+  const void* dev;
   hipStream_t stream;
   template <class P, class G, class C> void operator()() const {
-    const int count = (int)b.tensor.size();
-    if (nt) PCCL_LAUNCH((k_adamw8<P, G, C, true>), dim3(b.items), dim3(kWave), 0, stream, t, count, h);
-    else PCCL_LAUNCH((k_adamw8<P, G, C, false>), dim3(b.items), dim3(kWave), 0, stream, t, count, h);
+    if (plan.kind == kAdamW)
+      each_launch<AdamTable>(plan, b, grads, dev, [&](const AdamTable& t, const Share& s) {
+        const unsigned lds = adamw_lds(plan, b);
+        if (plan.stream) PCCL_LAUNCH((k_adamw<P, G, C, true>), dim3(s.items), dim3(kWave), lds, stream, t, s.dev, s.count, h);
+        else PCCL_LAUNCH((k_adamw<P, G, C, false>), dim3(s.items), dim3(kWave), lds, stream, t, s.dev, s.count, h);
+      });
+    else
+      each_launch<Adam8Table>(plan, b, grads, dev, [&](const Adam8Table& t, const Share& s) {
+        if (plan.stream) PCCL_LAUNCH((k_adamw8<P, G, C, true>), dim3(s.items), dim3(kWave), 0, stream, t, s.dev, s.count, h);
+        else PCCL_LAUNCH((k_adamw8<P, G, C, false>), dim3(s.items), dim3(kWave), 0, stream, t, s.dev, s.count, h);
+      });
   }
 };
 
@@ -356,40 +438,24 @@ template <class F> void with_type(int dtype, F&& f) {
 }
 
 struct BlocksLaunch {
-  const BlocksTable& t;
+  const pccl_optim_plan& plan;
   const Batch& b;
-  bool quantize, nt;
-  int root;
   hipStream_t stream;
   template <class T> void operator()() const {
-    const int count = (int)b.tensor.size();
-    if (quantize) {
-      if (nt) PCCL_LAUNCH((k_quantize<T, true>), dim3(b.items), dim3(kWave), 0, stream, t, count, root);
-      else PCCL_LAUNCH((k_quantize<T, false>), dim3(b.items), dim3(kWave), 0, stream, t, count, root);
-    } else {
-      if (nt) PCCL_LAUNCH((k_dequantize<T, true>), dim3(b.items), dim3(kWave), 0, stream, t, count, root);
-      else PCCL_LAUNCH((k_dequantize<T, false>), dim3(b.items), dim3(kWave), 0, stream, t, count, root);
-    }
+    constexpr int U = sizeof(typename T::elem) == 4 ? kQuantizeWide : kQuantizeNarrow;
+    each_launch<BlocksTable>(plan, b, nullptr, nullptr, [&](const BlocksTable& t, const Share& s) {
+      if (plan.kind == kQuantize) {
+        if (plan.stream) PCCL_LAUNCH((k_quantize<T, U, true>), dim3(s.items), dim3(kWave), 0, stream, t, s.count, plan.root);
+        else PCCL_LAUNCH((k_quantize<T, U, false>), dim3(s.items), dim3(kWave), 0, stream, t, s.count, plan.root);
+      } else {
+        if (plan.stream) PCCL_LAUNCH((k_dequantize<T, kDequantizeBlocks, true>), dim3(s.items), dim3(kWave), 0, stream, t, s.count, plan.root);
+        else PCCL_LAUNCH((k_dequantize<T, kDequantizeBlocks, false>), dim3(s.items), dim3(kWave), 0, stream, t, s.count, plan.root);
+      }
+    });
   }
 };
 
-struct NormLaunch {
-  const NormTable& t;
-  const Batch& b;
-  uint32_t grid;
-  bool nt, only;
-  double* part;
-  float* out;
-  hipStream_t stream;
-  template <class T> void operator()() const {
-    const int count = (int)b.tensor.size();
-    if (only) PCCL_LAUNCH((k_sum_squares<T, false, true>), dim3(grid), dim3(kNormThreads), 0, stream, t, count, b.items, part, out);
-    else if (nt) PCCL_LAUNCH((k_sum_squares<T, true, false>), dim3(grid), dim3(kNormThreads), 0, stream, t, count, b.items, part, out);
-    else PCCL_LAUNCH((k_sum_squares<T, false, false>), dim3(grid), dim3(kNormThreads), 0, stream, t, count, b.items, part, out);
-  }
-};
-
-uint32_t norm_grid(const Batch& b) { return b.items < kNormGroups ? b.items : kNormGroups; }
+uint32_t norm_grid(uint32_t items) { return std::min<uint32_t>((items + kNormThreads / kWave - 1) / (kNormThreads / kWave), kNormGroups); }
 
 // One workgroup does the whole norm where that takes less time than a second launch.
 constexpr uint32_t kNormAlone = 16;   // work items
@@ -398,9 +464,28 @@ bool norm_alone(const pccl_optim_plan& plan) { return plan.batches.size() == 1 &
 uint32_t norm_parts(const pccl_optim_plan& plan) {
   if (norm_alone(plan)) return 0;
   uint32_t parts = 0;
-  for (const Batch& b : plan.batches) parts += norm_grid(b);
+  for (const Batch& b : plan.batches) parts += norm_grid(b.items);
   return parts;
 }
+
+struct NormLaunch {
+  const pccl_optim_plan& plan;
+  const Batch& b;
+  double* part;
+  float* out;
+  hipStream_t stream;
+  template <class T> void operator()() const {
+    // a batch of a norm is never longer than a table in kernel arguments
+    each_launch<NormTable>(plan, b, nullptr, nullptr, [&](const NormTable& t, const Share& s) {
+      if (norm_alone(plan))
+        PCCL_LAUNCH((k_sum_squares<T, kNormThreads, false, true>), dim3(1), dim3(kNormThreads), 0, stream, t, s.count, s.items, part, out);
+      else if (plan.stream)
+        PCCL_LAUNCH((k_sum_squares<T, kNormThreads, true, false>), dim3(norm_grid(s.items)), dim3(kNormThreads), 0, stream, t, s.count, s.items, part, out);
+      else
+        PCCL_LAUNCH((k_sum_squares<T, kNormThreads, false, false>), dim3(norm_grid(s.items)), dim3(kNormThreads), 0, stream, t, s.count, s.items, part, out);
+    });
+  }
+};
 
 int check_plan(const pccl_optim_plan* plan, const char* what, Kind a, Kind b) {
   if (!plan) return fail(PCCL_HIP_EINVAL, "%s: plan is NULL", what);
@@ -429,7 +514,10 @@ int plan_blocks(pccl_optim_plan** out, Kind kind, const void* const* codes, cons
       plan.b.push_back((void*)scales[i]);
       plan.c.push_back((void*)x[i]);
     }
-    return make_batches(plan, dtype, nullptr, nullptr, kBlock, kBlockSegs, what);
+    auto items = [&](int i) {
+      return items_for(n[i], (size_t)kBlock * (!q ? kDequantizeBlocks : esize_of(dtype[i]) == 4 ? kQuantizeWide : kQuantizeNarrow));
+    };
+    return make_batches(plan, dtype, nullptr, nullptr, items, BlocksTable::kInline, what);
   });
 }
 
@@ -446,7 +534,7 @@ int pccl_optim_plan_adamw(pccl_optim_plan** plan, void* const* params, const voi
                           const int* grad_dtype, const int* copy_dtype, int count) {
   return new_plan(plan, kAdamW, count, n, "pccl_optim_plan_adamw", [&](pccl_optim_plan& p, Checker& check) {
     return make_adamw(p, check, params, grads, exp_avg, exp_avg_sq, nullptr, nullptr, copies, param_dtype, grad_dtype,
-                      copy_dtype, (size_t)kAdamUnroll * kBlock, kAdamSegs);
+                      copy_dtype);
   });
 }
 
@@ -456,14 +544,34 @@ int pccl_optim_plan_adamw8(pccl_optim_plan** plan, void* const* params, const vo
                            const int* copy_dtype, int count) {
   return new_plan(plan, kAdamW8, count, n, "pccl_optim_plan_adamw8", [&](pccl_optim_plan& p, Checker& check) {
     return make_adamw(p, check, params, grads, exp_avg, exp_avg_rms, avg_scale, rms_scale, copies, param_dtype, grad_dtype,
-                      copy_dtype, kBlock, kAdam8Segs);
+                      copy_dtype);
   });
 }
 
-int pccl_optim_run_adamw(const pccl_optim_plan* plan, const void* const* grads, const pccl_optim_step* step, void* stream) {
+size_t pccl_optim_table_bytes(const pccl_optim_plan* plan) {
+  if (!plan) return 0;
+  return plan->kind == kAdamW ? table_bytes<AdamTable>(*plan) : plan->kind == kAdamW8 ? table_bytes<Adam8Table>(*plan) : 0;
+}
+
+int pccl_optim_table_fill(const pccl_optim_plan* plan, void* host, size_t bytes) {
+  const char* what = "pccl_optim_table_fill";
+  if (int rc = check_plan(plan, what, kAdamW, kAdamW8)) return rc;
+  const size_t need = pccl_optim_table_bytes(plan);
+  if (!need) return PCCL_HIP_OK;
+  if (!host || bytes < need) return fail(PCCL_HIP_EINVAL, "%s: needs %zu bytes, got %zu", what, need, host ? bytes : (size_t)0);
+  memset(host, 0, need);
+  if (plan->kind == kAdamW) table_fill<AdamTable>(*plan, (char*)host);
+  else table_fill<Adam8Table>(*plan, (char*)host);
+  return PCCL_HIP_OK;
+}
+
+int pccl_optim_run_adamw(const pccl_optim_plan* plan, const void* const* grads, const void* table, const pccl_optim_step* step,
+                         void* stream) {
   const char* what = "pccl_optim_run_adamw";
   if (int rc = check_plan(plan, what, kAdamW, kAdamW8)) return rc;
   if (!step) return fail(PCCL_HIP_EINVAL, "%s: step is NULL", what);
+  if (table && !pccl_optim_table_bytes(plan)) return fail(PCCL_HIP_EINVAL, "%s: this plan has no table", what);
+  if ((uintptr_t)table % 64) return fail(PCCL_HIP_EINVAL, "%s: table is not aligned to 64 bytes", what);
   Hyper h;
   if (int rc = make_hyper(*plan, *step, h, what)) return rc;
   if (grads)
@@ -475,28 +583,10 @@ int pccl_optim_run_adamw(const pccl_optim_plan* plan, const void* const* grads, 
         return fail(PCCL_HIP_EINVAL, "%s: grads[%d] is not aligned to its element size (%zu bytes)", what, i, es);
       if (int rc = check_apart(*plan, grads[i], plan->n[i] * es, "grads", i, what)) return rc;
     }
+  const char* dev = grads ? nullptr : (const char*)table;
   for (const Batch& b : plan->batches) {
-    const int count = (int)b.tensor.size();
-    if (plan->kind == kAdamW) {
-      AdamTable t;
-      for (int k = 0; k < count; ++k) {
-        const int i = b.tensor[k];
-        t.p[k] = plan->a[i]; t.g[k] = grads ? grads[i] : plan->g[i];
-        t.m[k] = plan->b[i]; t.v[k] = plan->c[i]; t.c[k] = plan->d[i];
-        t.n[k] = plan->n[i]; t.start[k] = b.start[k];
-      }
-      with_types(b, AdamLaunch{t, b, h, plan->stream, (hipStream_t)stream});
-    } else {
-      Adam8Table t;
-      for (int k = 0; k < count; ++k) {
-        const int i = b.tensor[k];
-        t.p[k] = plan->a[i]; t.g[k] = grads ? grads[i] : plan->g[i];
-        t.m[k] = plan->b[i]; t.r[k] = plan->c[i]; t.c[k] = plan->d[i];
-        t.ms[k] = (float*)plan->e[i]; t.rs[k] = (float*)plan->f[i];
-        t.n[k] = plan->n[i]; t.start[k] = b.start[k];
-      }
-      with_types(b, Adam8Launch{t, b, h, plan->stream, (hipStream_t)stream});
-    }
+    with_types(b, AdamLaunch{*plan, b, h, grads, dev, (hipStream_t)stream});
+    if (dev) dev += plan->kind == kAdamW ? table_size<AdamEntry>(b) : table_size<Adam8Entry>(b);
   }
   return launch_status(what);
 }
@@ -511,7 +601,8 @@ int pccl_optim_plan_norm(pccl_optim_plan** plan, const void* const* tensors, con
       if ((rc = check.buffer(tensors[i], n[i] * esize_of(dtype[i]), esize_of(dtype[i]), "tensors", i, false))) return rc;
       p.g.push_back(tensors[i]);
     }
-    return make_batches(p, dtype, nullptr, nullptr, kNormTile, kNormSegs, what);
+    return make_batches(p, dtype, nullptr, nullptr, [&](int i) { return items_for(n[i] * esize_of(dtype[i]), kNormBytes); },
+                        NormTable::kInline, what);
   });
 }
 
@@ -528,18 +619,13 @@ int pccl_optim_run_norm(const pccl_optim_plan* plan, float* out, void* work, siz
   if (need && (!work || work_bytes < need))
     return fail(PCCL_HIP_EINVAL, "%s: needs %zu bytes of work space, got %zu", what, need, work ? work_bytes : (size_t)0);
   if (need && (uintptr_t)work % sizeof(double)) return fail(PCCL_HIP_EINVAL, "%s: work is not aligned to 8 bytes", what);
-  const bool only = norm_alone(*plan);
   double* part = (double*)work;
   for (const Batch& b : plan->batches) {
-    NormTable t;
-    for (size_t k = 0; k < b.tensor.size(); ++k) {
-      t.x[k] = plan->g[b.tensor[k]]; t.n[k] = plan->n[b.tensor[k]]; t.start[k] = b.start[k];
-    }
-    const uint32_t grid = only ? 1 : norm_grid(b);
-    with_type(b.p, NormLaunch{t, b, grid, plan->stream, only, part, out, (hipStream_t)stream});
-    part += grid;
+    with_type(b.p, NormLaunch{*plan, b, part, out, (hipStream_t)stream});
+    part += norm_grid(b.items);
   }
-  if (!only) PCCL_LAUNCH(k_norm_join, dim3(1), dim3(kNormThreads), 0, (hipStream_t)stream, (const double*)work, norm_parts(*plan), out);
+  if (!norm_alone(*plan))
+    PCCL_LAUNCH(k_norm_join, dim3(1), dim3(kWave), 0, (hipStream_t)stream, (const double*)work, norm_parts(*plan), out);
   return launch_status(what);
 }
 
@@ -556,15 +642,7 @@ int pccl_optim_plan_dequantize(pccl_optim_plan** plan, void* const* dst, const v
 int pccl_optim_run_blocks(const pccl_optim_plan* plan, void* stream) {
   const char* what = "pccl_optim_run_blocks";
   if (int rc = check_plan(plan, what, kQuantize, kDequantize)) return rc;
-  for (const Batch& b : plan->batches) {
-    BlocksTable t;
-    for (size_t k = 0; k < b.tensor.size(); ++k) {
-      const int i = b.tensor[k];
-      t.codes[k] = plan->a[i]; t.scales[k] = (float*)plan->b[i]; t.x[k] = plan->c[i];
-      t.n[k] = plan->n[i]; t.start[k] = b.start[k];
-    }
-    with_type(b.p, BlocksLaunch{t, b, plan->kind == kQuantize, plan->stream, plan->root, (hipStream_t)stream});
-  }
+  for (const Batch& b : plan->batches) with_type(b.p, BlocksLaunch{*plan, b, (hipStream_t)stream});
   return launch_status(what);
 }
 

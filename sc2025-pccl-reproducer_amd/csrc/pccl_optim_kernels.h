@@ -31,17 +31,10 @@ constexpr int kVec = 4;                     // elements of a lane
 constexpr int kBlock = kWave * kVec;        // elements of a wave, and of a block of the 8-bit form
 static_assert(kBlock == PCCL_OPTIM_BLOCK, "a wave holds one block");
 
-// Tensors of one launch: their addresses travel in the kernel arguments, which
-// are kept below 4 KiB.
-constexpr int kAdamSegs = 64;               // 52 bytes each
-constexpr int kAdam8Segs = 56;              // 68 bytes each
-constexpr int kNormSegs = 64;
-constexpr int kBlockSegs = 64;
-
 constexpr float kCodeMax = 448.0f;              // largest finite e4m3 value
 constexpr float kCodeMin = 0x1p-9f;             // smallest positive one
 constexpr float kCodeNormal = 0x1p-6f;          // smallest with a full mantissa
-constexpr float kAmaxFloor = 0x1p-100f;         // keeps 1 / scale finite for blocks of zeros and denormals
+constexpr uint32_t kFloorBits = 0x0d800000u;    // 2^-100: keeps 1 / scale finite for blocks of zeros and denormals
 
 // ---------------------------------------------------------------------------
 // lanes
@@ -55,6 +48,15 @@ constexpr bool kHostRun = true;
 constexpr int kLaneSlots = kWave;
 template <class F> __device__ __forceinline__ void each_lane(F&& f) { for (int l = 0; l < kWave; ++l) f(l, l); }
 #endif
+
+// A value that the caller knows to be the same in all lanes, for the compiler
+__device__ __forceinline__ uint32_t wave_uniform(uint32_t x) {
+#if defined(__HIP_DEVICE_COMPILE__)
+  return (uint32_t)__builtin_amdgcn_readfirstlane((int)x);
+#else
+  return x;
+#endif
+}
 
 // Largest of an unsigned value over the wave, in every lane.  Six DPP steps
 // (shifts within rows of 16, then the row results handed on), no LDS.
@@ -81,18 +83,80 @@ __device__ __forceinline__ uint32_t wave_max(const uint32_t* lanes) {
 #endif
 }
 
-// The tensor that work item `item` belongs to: start[] holds the first item of
-// each of the `count` <= 64 tensors, in rising order from 0.  Every lane
-// compares one entry; the number of starts at or below the item is the answer.
-__device__ __forceinline__ int find_segment(const uint32_t* start, int count, uint32_t item) {
+// ---------------------------------------------------------------------------
+// the tensors of a launch
+// ---------------------------------------------------------------------------
+// start[] holds the first work item of each tensor, in rising order from 0.  The
+// table travels in the kernel arguments, which are kept below 4 KiB, or lies in
+// device memory, where one launch then serves up to kTableMax tensors.
+template <class E, int CAP> struct Table {
+  typedef E entry;
+  static constexpr int kInline = CAP;
+  E e[CAP];
+  uint32_t start[CAP];
+};
+constexpr int kTableMax = kWave * kWave;
+
+struct AdamEntry { void* p; const void* g; void* m; void* v; void* c; size_t n; };
+struct Adam8Entry { void* p; const void* g; void* m; void* r; float* ms; float* rs; void* c; size_t n; };
+struct BlocksEntry { void* codes; float* scales; void* x; size_t n; };
+struct NormEntry { const void* x; size_t n; };
+typedef Table<AdamEntry, 64> AdamTable;
+typedef Table<Adam8Entry, 56> Adam8Table;
+typedef Table<BlocksEntry, 104> BlocksTable;
+typedef Table<NormEntry, 192> NormTable;
+
+// Both places are read through the constant address space, i.e. by scalar loads:
+// nothing writes a table while a kernel runs.
+#if defined(__HIP_DEVICE_COMPILE__)
+#define PCCL_CONSTANT __attribute__((address_space(4)))
+#define PCCL_GLOBAL __attribute__((address_space(1)))
+#else
+#define PCCL_CONSTANT
+#define PCCL_GLOBAL
+#endif
+// Addresses read from a table are said to be of global memory: to the compiler
+// they could be anything, and it would use flat accesses.
+typedef PCCL_GLOBAL char* gptr;
+typedef const PCCL_GLOBAL char* cgptr;
+
+template <class E> struct View {
+  const PCCL_CONSTANT E* e;
+  const PCCL_CONSTANT uint32_t* start;
+};
+
+// The table is the kernel's FIRST argument, i.e. at the start of its arguments.
+template <class T> __device__ __forceinline__ View<typename T::entry> view_of(const T& args, const void* dev, int count) {
+  typedef typename T::entry E;
+#if defined(__HIP_DEVICE_COMPILE__)
+  typedef const PCCL_CONSTANT char* bytes;
+  const bytes in_args = (bytes)__builtin_amdgcn_kernarg_segment_ptr(), in_memory = (bytes)(uintptr_t)dev;
+  const bytes entries = dev ? in_memory : in_args;
+  return {(const PCCL_CONSTANT E*)entries,
+          (const PCCL_CONSTANT uint32_t*)(entries + (dev ? (size_t)count * sizeof(E) : offsetof(T, start)))};
+#else
+  if (!dev) return {args.e, args.start};
+  return {(const E*)dev, (const uint32_t*)((const char*)dev + (size_t)count * sizeof(E))};
+#endif
+}
+
+// The tensor that a work item belongs to: every lane compares one start, and the
+// number of those at or below the item is the answer; above 64 tensors first
+// among every 64th.
+template <class E> __device__ __forceinline__ int find_segment(const View<E>& v, int count, uint32_t item) {
   if (count == 1) return 0;
 #if defined(__HIP_DEVICE_COMPILE__)
   const int lane = (int)(threadIdx.x & (kWave - 1));
-  const uint64_t at = __builtin_amdgcn_ballot_w64(lane < count && start[lane < count ? lane : 0] <= item);
-  return __builtin_popcountll(at) - 1;
+  int base = 0;
+  if (count > kWave) {
+    const int at = lane * kWave;
+    base = (__builtin_popcountll(__builtin_amdgcn_ballot_w64(at < count && v.start[at < count ? at : 0] <= item)) - 1) * kWave;
+  }
+  const int at = base + lane;
+  return base + __builtin_popcountll(__builtin_amdgcn_ballot_w64(at < count && v.start[at < count ? at : 0] <= item)) - 1;
 #else
   int s = 0;
-  while (s + 1 < count && start[s + 1] <= item) ++s;
+  while (s + 1 < count && v.start[s + 1] <= item) ++s;
   return s;
 #endif
 }
@@ -102,41 +166,50 @@ __device__ __forceinline__ int find_segment(const uint32_t* start, int count, ui
 // gfx950 takes vector accesses at any alignment; a tensor that starts in the
 // middle of a flat buffer runs in the same code as an aligned one.
 // ---------------------------------------------------------------------------
-typedef uint32_t u32x4a __attribute__((ext_vector_type(4), aligned(4)));
+typedef uint32_t u32x4a __attribute__((ext_vector_type(4), aligned(2)));
 typedef uint32_t u32x2a __attribute__((ext_vector_type(2), aligned(2)));
 typedef uint32_t u32a __attribute__((aligned(1)));
 
 // NT: with the non-temporal hint (the alignment belongs to the pointed-to type, so these are not one template)
-template <bool NT> __device__ __forceinline__ u32x4a load16(const void* p) {
-  if constexpr (NT) return __builtin_nontemporal_load((const u32x4a*)p);
-  else return *(const u32x4a*)p;
+template <bool NT> __device__ __forceinline__ u32x4a load16(cgptr p) {
+  if constexpr (NT) return __builtin_nontemporal_load((const PCCL_GLOBAL u32x4a*)p);
+  else return *(const PCCL_GLOBAL u32x4a*)p;
 }
-template <bool NT> __device__ __forceinline__ u32x2a load8(const void* p) {
-  if constexpr (NT) return __builtin_nontemporal_load((const u32x2a*)p);
-  else return *(const u32x2a*)p;
+template <bool NT> __device__ __forceinline__ u32x2a load8(cgptr p) {
+  if constexpr (NT) return __builtin_nontemporal_load((const PCCL_GLOBAL u32x2a*)p);
+  else return *(const PCCL_GLOBAL u32x2a*)p;
 }
-template <bool NT> __device__ __forceinline__ void store16(void* p, u32x4a v) {
-  if constexpr (NT) __builtin_nontemporal_store(v, (u32x4a*)p);
-  else *(u32x4a*)p = v;
+template <bool NT> __device__ __forceinline__ uint32_t load4b(cgptr p) {
+  if constexpr (NT) return __builtin_nontemporal_load((const PCCL_GLOBAL u32a*)p);
+  else return *(const PCCL_GLOBAL u32a*)p;
 }
-template <bool NT> __device__ __forceinline__ void store8(void* p, u32x2a v) {
-  if constexpr (NT) __builtin_nontemporal_store(v, (u32x2a*)p);
-  else *(u32x2a*)p = v;
+template <bool NT> __device__ __forceinline__ void store16(gptr p, u32x4a v) {
+  if constexpr (NT) __builtin_nontemporal_store(v, (PCCL_GLOBAL u32x4a*)p);
+  else *(PCCL_GLOBAL u32x4a*)p = v;
+}
+template <bool NT> __device__ __forceinline__ void store8(gptr p, u32x2a v) {
+  if constexpr (NT) __builtin_nontemporal_store(v, (PCCL_GLOBAL u32x2a*)p);
+  else *(PCCL_GLOBAL u32x2a*)p = v;
+}
+template <bool NT> __device__ __forceinline__ void store4b(gptr p, uint32_t v) {
+  if constexpr (NT) __builtin_nontemporal_store(v, (PCCL_GLOBAL u32a*)p);
+  else *(PCCL_GLOBAL u32a*)p = v;
 }
 
+// i: place relative to p, in elements
 struct F32 {
   typedef float elem;
   static constexpr bool kNone = false;
-  template <bool NT> static __device__ __forceinline__ void load4(const void* p, size_t i, float* x) {
-    const u32x4a w = load16<NT>((const elem*)p + i);
+  template <bool NT> static __device__ __forceinline__ void load4(cgptr p, uint32_t i, float* x) {
+    const u32x4a w = load16<NT>(p + i * 4u);
     x[0] = __uint_as_float(w.x); x[1] = __uint_as_float(w.y); x[2] = __uint_as_float(w.z); x[3] = __uint_as_float(w.w);
   }
-  template <bool NT> static __device__ __forceinline__ void store4(void* p, size_t i, const float* x) {
+  template <bool NT> static __device__ __forceinline__ void store4(gptr p, uint32_t i, const float* x) {
     const u32x4a w = {__float_as_uint(x[0]), __float_as_uint(x[1]), __float_as_uint(x[2]), __float_as_uint(x[3])};
-    store16<NT>((elem*)p + i, w);
+    store16<NT>(p + i * 4u, w);
   }
-  static __device__ __forceinline__ float load1(const void* p, size_t i) { return ((const elem*)p)[i]; }
-  static __device__ __forceinline__ void store1(void* p, size_t i, float x) { ((elem*)p)[i] = x; }
+  static __device__ __forceinline__ float load1(cgptr p, uint32_t i) { return ((const PCCL_GLOBAL elem*)p)[i]; }
+  static __device__ __forceinline__ void store1(gptr p, uint32_t i, float x) { ((PCCL_GLOBAL elem*)p)[i] = x; }
 };
 
 // T: __bf16 or _Float16; the conversions round to nearest even
@@ -145,41 +218,71 @@ template <class T> struct Half {
   static constexpr bool kNone = false;
   typedef T x4 __attribute__((ext_vector_type(4)));
   typedef float f4 __attribute__((ext_vector_type(4)));
-  template <bool NT> static __device__ __forceinline__ void load4(const void* p, size_t i, float* x) {
-    const u32x2a w = load8<NT>((const elem*)p + i);
+  template <bool NT> static __device__ __forceinline__ void load4(cgptr p, uint32_t i, float* x) {
+    const u32x2a w = load8<NT>(p + i * 2u);
     x4 h;
     __builtin_memcpy(&h, &w, 8);
     const f4 f = __builtin_convertvector(h, f4);
     x[0] = f.x; x[1] = f.y; x[2] = f.z; x[3] = f.w;
   }
-  template <bool NT> static __device__ __forceinline__ void store4(void* p, size_t i, const float* x) {
+  template <bool NT> static __device__ __forceinline__ void store4(gptr p, uint32_t i, const float* x) {
     const f4 f = {x[0], x[1], x[2], x[3]};
     const x4 h = __builtin_convertvector(f, x4);
     u32x2a w;
     __builtin_memcpy(&w, &h, 8);
-    store8<NT>((elem*)p + i, w);
+    store8<NT>(p + i * 2u, w);
   }
-  static __device__ __forceinline__ float load1(const void* p, size_t i) { return (float)((const elem*)p)[i]; }
-  static __device__ __forceinline__ void store1(void* p, size_t i, float x) { ((elem*)p)[i] = (elem)x; }
+  static __device__ __forceinline__ float load1(cgptr p, uint32_t i) { return (float)((const PCCL_GLOBAL elem*)p)[i]; }
+  static __device__ __forceinline__ void store1(gptr p, uint32_t i, float x) { ((PCCL_GLOBAL elem*)p)[i] = (elem)x; }
 };
 typedef Half<__bf16> BF16;
 typedef Half<_Float16> F16;
 
 struct None {   // no copy
   static constexpr bool kNone = true;
-  template <bool NT> static __device__ __forceinline__ void store4(void*, size_t, const float*) {}
-  static __device__ __forceinline__ void store1(void*, size_t, float) {}
 };
 
-// Elements [i, i + 4) of a tensor of n; what lies behind its end is 0 and is
-// not stored.
-template <class T, bool NT> __device__ __forceinline__ void load_upto4(const void* p, size_t i, size_t n, float* x) {
-  if (i + kVec <= n) { T::template load4<NT>(p, i, x); return; }
-  for (int e = 0; e < kVec; ++e) x[e] = i + e < n ? T::load1(p, i + e) : 0.0f;
+// The elements [lo, hi) of a work item that are its tensor's.  A work item is
+// addressed by its first element (the same for the whole wave, so it stays in
+// scalar registers) and 32-bit places relative to it.
+struct Span { uint32_t lo, hi; };
+__device__ __forceinline__ bool whole4(uint32_t i, Span s) { return i >= s.lo && i + kVec <= s.hi; }
+__device__ __forceinline__ bool inside(uint32_t i, Span s) { return i >= s.lo && i < s.hi; }
+
+// Elements [i, i + 4) of an item; those outside the span are 0 and are not
+// stored.  FULL: the caller knows that all four are inside.
+template <class T, bool NT, bool FULL> __device__ __forceinline__ void load_upto4(cgptr p, uint32_t i, Span s, float* x) {
+  if (FULL || whole4(i, s)) { T::template load4<NT>(p, i, x); return; }
+  for (int e = 0; e < kVec; ++e) x[e] = inside(i + e, s) ? T::load1(p, i + e) : 0.0f;
 }
-template <class T, bool NT> __device__ __forceinline__ void store_upto4(void* p, size_t i, size_t n, const float* x) {
-  if (i + kVec <= n) { T::template store4<NT>(p, i, x); return; }
-  for (int e = 0; e < kVec; ++e) if (i + e < n) T::store1(p, i + e, x[e]);
+template <class T, bool NT, bool FULL> __device__ __forceinline__ void store_upto4(gptr p, uint32_t i, Span s, const float* x) {
+  if (FULL || whole4(i, s)) { T::template store4<NT>(p, i, x); return; }
+  for (int e = 0; e < kVec; ++e) if (inside(i + e, s)) T::store1(p, i + e, x[e]);
+}
+
+// Address of an element of a tensor, `at` possibly before its start
+__device__ __forceinline__ gptr element(const void* p, ptrdiff_t at, size_t bytes) {
+  return (gptr)((uintptr_t)p + (uintptr_t)at * bytes);
+}
+
+// The smaller of the two.  In halves: the compiler has left a 64-bit comparison
+// of this form in the vector unit and its selection in the scalar unit, which
+// then read a condition that nobody had set.
+__device__ __forceinline__ uint32_t at_most(size_t rest, uint32_t size) {
+  const uint32_t low = (uint32_t)rest;
+  return (uint32_t)((uint64_t)rest >> 32) != 0 || low > size ? size : low;
+}
+
+// What a work item of `size` elements that starts at element `first` of n has of its tensor
+__device__ __forceinline__ Span span_of(size_t first, size_t n, uint32_t size) { return {0, at_most(n - first, size)}; }
+
+// f(true_type) for a work item that lies whole in its tensor, which runs without
+// a bound check, f(false_type) for the last one.  The choice is the same for the
+// whole wave.
+template <bool V> struct Full { static constexpr bool value = V; };
+template <class F> __device__ __forceinline__ void with_bounds(bool full, F&& f) {
+  if (full) f(Full<true>());
+  else f(Full<false>());
 }
 
 // ---------------------------------------------------------------------------
@@ -200,7 +303,9 @@ __device__ __forceinline__ void decode4(uint32_t w, float* x) {
 #endif
 }
 
-// |x| <= 448 (1 + 2^-20) or NaN: nothing here overflows
+// To nearest, ties to even.  |x| <= 448 (1 + 2^-20): nothing here overflows.  (A
+// block with an inf or NaN has a scale that is not finite: its codes do not
+// matter.)
 __device__ __forceinline__ uint32_t encode4(const float* x) {
 #if defined(__HIP_DEVICE_COMPILE__)
   int w = __builtin_amdgcn_cvt_pk_fp8_f32(x[0], x[1], 0, false);
@@ -209,9 +314,8 @@ __device__ __forceinline__ uint32_t encode4(const float* x) {
   uint32_t w = 0;
   for (int e = 0; e < 4; ++e) {
     const float a = std::fabs(x[e]);
-    uint32_t c;
-    if (!(a == a)) c = 0x7f;
-    else {
+    uint32_t c = 0x7f;
+    if (a < 480.0f) {
       int ex = 0;
       std::frexp(a, &ex);
       if (a == 0 || ex < -5) ex = -5;
@@ -224,6 +328,40 @@ __device__ __forceinline__ uint32_t encode4(const float* x) {
 #endif
 }
 
+// A value that a carry would take out of the codes: 448 times 1 + 2^-20
+__device__ __forceinline__ float clamp_code(float x) {
+#if defined(__HIP_DEVICE_COMPILE__)
+  return __builtin_amdgcn_fmed3f(x, -kCodeMax, kCodeMax);
+#else
+  return x > kCodeMax ? kCodeMax : x < -kCodeMax ? -kCodeMax : x;
+#endif
+}
+
+// |x| <= 448.  To one of the two codes next to x, the upper one (in magnitude) with the
+// probability of its nearness: the 16 random bits in the upper half of each
+// bits[e] are added to the 20 mantissa bits that e4m3 drops, which are then cut
+// off; below 2^-6, where the codes are 2^-9 apart, to x in units of that.  It is
+// what v_cvt_sr_fp8_f32 does with its second operand's upper 20 bits (checked on
+// MI355X against this description for 4 million values and random numbers).
+__device__ __forceinline__ uint32_t encode4_stochastic(const float* x, const uint32_t* bits) {
+  uint32_t w = 0;
+#if defined(__HIP_DEVICE_COMPILE__)
+  w = (uint32_t)__builtin_amdgcn_cvt_sr_fp8_f32(x[0], (int)bits[0], (int)w, 0);
+  w = (uint32_t)__builtin_amdgcn_cvt_sr_fp8_f32(x[1], (int)bits[1], (int)w, 1);
+  w = (uint32_t)__builtin_amdgcn_cvt_sr_fp8_f32(x[2], (int)bits[2], (int)w, 2);
+  w = (uint32_t)__builtin_amdgcn_cvt_sr_fp8_f32(x[3], (int)bits[3], (int)w, 3);
+#else
+  float y[kVec];
+  for (int e = 0; e < 4; ++e) {
+    const float a = std::fabs(x[e]), shift = a < kCodeNormal ? kCodeNormal : 0.0f;
+    const float q = __uint_as_float((__float_as_uint(a + shift) + (bits[e] >> 12)) & 0xfff00000u) - shift;
+    y[e] = std::copysign(q, x[e]);
+  }
+  w = encode4(y);
+#endif
+  return w;
+}
+
 // A 32-bit multiply-xorshift mix; the multipliers are from Chris Wellons'
 // public-domain search for mixes of this form with low bias.
 __device__ __forceinline__ uint32_t mix32(uint32_t x) {
@@ -232,34 +370,32 @@ __device__ __forceinline__ uint32_t mix32(uint32_t x) {
   return x ^ (x >> 16);
 }
 __device__ __forceinline__ uint32_t noise_key(uint32_t seed, uint64_t step) { return mix32(mix32(seed) + (uint32_t)step); }
-__device__ __forceinline__ uint32_t noise(uint32_t key, uint64_t index) {
-  return mix32((uint32_t)index + key + (uint32_t)(index >> 32) * 0x9e3779b1u);
-}
-
-// y, |y| <= 448 (1 + 2^-20), to one of the two e4m3 values next to it, the upper
-// one with the probability of its nearness: 16 random bits are added to the 20
-// mantissa bits that e4m3 drops, which are then cut off.  Below 2^-6 the codes
-// are 2^-9 apart, as they are just above it, so the value is moved up there and
-// back.  The result is exactly a code.  NaN stays NaN (a carry out of its
-// mantissa is kept out by the test).
-__device__ __forceinline__ float round_stochastic(float y, uint32_t u16) {
-  const float a = std::fabs(y);
-  const float shift = a < kCodeNormal ? kCodeNormal : 0.0f;
-  const uint32_t cut = (__float_as_uint(a + shift) + (u16 << 4)) & 0xfff00000u;
-  const float q = __uint_as_float(cut) - shift;
-  return std::copysign(a <= kCodeMax * 1.001f ? (q > kCodeMax ? kCodeMax : q) : y, y);
+// 32 random bits for an element of the block that starts at `first` (a multiple
+// of 256, so the upper half of the index is that of the whole block)
+__device__ __forceinline__ uint32_t noise(uint32_t key, size_t first, uint32_t i) {
+  return mix32((uint32_t)first + key + (uint32_t)((uint64_t)first >> 32) * 0x9e3779b1u + i);
 }
 
 struct BlockScale { float scale, inv; };
+constexpr float kInvCodeMax = 1.0f / kCodeMax;   // 448 times it is exactly 1
 
-// From the largest |x| of a block, as bits (NaN is above infinity there, and
-// comes out as NaN).
+// 1 / x for a normal x whose reciprocal is normal: the hardware's, good to one
+// unit in the last place, and one Newton step, which makes it the rounded one.
+__device__ __forceinline__ float reciprocal(float x) {
+#if defined(__HIP_DEVICE_COMPILE__)
+  const float r = __builtin_amdgcn_rcpf(x);
+  return __builtin_fmaf(__builtin_fmaf(-x, r, 1.0f), r, r);
+#else
+  return 1.0f / x;
+#endif
+}
+
+// From the largest |x| of a block, as bits.  The comparison is one of integers,
+// in which NaN is above infinity, so that either becomes the scale.
 __device__ __forceinline__ BlockScale block_scale(uint32_t amax_bits) {
-  float a = __uint_as_float(amax_bits);
-  a = a < kAmaxFloor ? kAmaxFloor : a;
   BlockScale s;
-  s.scale = a / kCodeMax;
-  s.inv = 1.0f / s.scale;
+  s.scale = __uint_as_float(amax_bits > kFloorBits ? amax_bits : kFloorBits) * kInvCodeMax;
+  s.inv = reciprocal(s.scale);
   return s;
 }
 
@@ -272,17 +408,25 @@ __device__ __forceinline__ uint32_t amax4(const float* x) {
   return a;
 }
 
-// A root other than 0 keeps at least the smallest code.
-__device__ __forceinline__ float lift_root(float r, float y) { return r > 0.0f && y < kCodeMin ? kCodeMin : y; }
-
-__device__ __forceinline__ void store_codes(void* p, size_t i, size_t n, uint32_t w) {
-  if (i + kVec <= n) { *(u32a*)((uint8_t*)p + i) = w; return; }
-  for (int e = 0; e < kVec; ++e) if (i + e < n) ((uint8_t*)p)[i + e] = (uint8_t)(w >> (8 * e));
+// y = r / scale, at least the smallest code for a root r other than 0 and at most
+// the largest: the middle one of y, 2^-9 and a number that is 0 for r = 0 and
+// beyond 448 for every other root (the smallest is 2^-74.5).
+__device__ __forceinline__ float lift_root(float r, float y) {
+#if defined(__HIP_DEVICE_COMPILE__)
+  return __builtin_amdgcn_fmed3f(y, kCodeMin, std::fmin(r * 0x1p100f, kCodeMax));
+#else
+  return r == 0 ? 0.0f : y < kCodeMin ? kCodeMin : y > kCodeMax ? kCodeMax : y;
+#endif
 }
-__device__ __forceinline__ uint32_t load_codes(const void* p, size_t i, size_t n) {
-  if (i + kVec <= n) return *(const u32a*)((const uint8_t*)p + i);
+
+template <bool NT, bool FULL> __device__ __forceinline__ void store_codes(gptr p, uint32_t i, Span s, uint32_t w) {
+  if (FULL || whole4(i, s)) { store4b<NT>(p + i, w); return; }
+  for (int e = 0; e < kVec; ++e) if (inside(i + e, s)) p[i + e] = (char)(w >> (8 * e));
+}
+template <bool NT, bool FULL> __device__ __forceinline__ uint32_t load_codes(cgptr p, uint32_t i, Span s) {
+  if (FULL || whole4(i, s)) return load4b<NT>(p + i);
   uint32_t w = 0;
-  for (int e = 0; e < kVec; ++e) if (i + e < n) w |= (uint32_t)((const uint8_t*)p)[i + e] << (8 * e);
+  for (int e = 0; e < kVec; ++e) if (inside(i + e, s)) w |= (uint32_t)(uint8_t)p[i + e] << (8 * e);
   return w;
 }
 
@@ -326,7 +470,7 @@ __device__ __forceinline__ void fill_schedule(Hyper& h, double lr, uint64_t t) {
 // Completes the scalars from device memory; false if the step is skipped.
 __device__ __forceinline__ bool finish_hyper(Hyper& h) {
   if (h.norm) {
-    const float norm = *h.norm;
+    const float norm = *(const PCCL_GLOBAL float*)(uintptr_t)h.norm;
     if (h.skip_nonfinite && !(std::fabs(norm) <= 3.402823466e38f)) return false;
     if (h.max_norm > 0.0f) {
       const float c = h.max_norm / (norm * std::fabs(h.grad_scale) + 1e-6f);
@@ -343,183 +487,255 @@ __device__ __forceinline__ bool finish_hyper(Hyper& h) {
   return true;
 }
 
-// One element.  Returns sqrt(v), which the 8-bit form stores.
-__device__ __forceinline__ float adamw_element(const Hyper& h, float& p, float g, float& m, float& v) {
-  g *= h.grad_scale;
-  m = h.beta1 * m + h.one_minus_beta1 * g;
-  v = h.beta2 * v + h.one_minus_beta2 * (g * g);
-  const float root = sqrtf(v);
-  const float update = m / (root * h.inv_root_bias + h.eps);
-  p -= h.lr_decay * p + h.step_size * update;   // the two small terms first: 1 - lr * decay would round them away
-  return root;
+// sqrt of four numbers >= 0.  For normal ones from the hardware's 1 / sqrt(x),
+// good to one unit in the last place, and a correction by the exact residue, a
+// third of the instructions of sqrtf: correctly rounded in all but about one of
+// a million cases.  Zeros, denormals, infinity and NaN go the long way.
+__device__ __forceinline__ void sqrt4(const float* x, float* root) {
+#if defined(__HIP_DEVICE_COMPILE__)
+  uint32_t top = 0;
+#pragma unroll
+  for (int e = 0; e < kVec; ++e) {
+    const uint32_t b = __float_as_uint(x[e]) - 0x00800000u;      // below 0x7f000000 for the normal ones alone
+    top = b > top ? b : top;
+  }
+  if (top < 0x7f000000u) {
+#pragma unroll
+    for (int e = 0; e < kVec; ++e) {
+      const float r = __builtin_amdgcn_rsqf(x[e]);
+      const float s = x[e] * r;
+      root[e] = __builtin_fmaf(__builtin_fmaf(-s, s, x[e]), 0.5f * r, s);
+    }
+    return;
+  }
+#endif
+#pragma unroll
+  for (int e = 0; e < kVec; ++e) root[e] = sqrtf(x[e]);
 }
 
-struct AdamTable {
-  void* p[kAdamSegs];
-  const void* g[kAdamSegs];
-  void* m[kAdamSegs];
-  void* v[kAdamSegs];
-  void* c[kAdamSegs];
-  size_t n[kAdamSegs];
-  uint32_t start[kAdamSegs];   // first workgroup of each tensor
-};
+// Four elements; v comes back as its root, too, which the 8-bit form stores.
+// The moments are computed without fused multiply-adds: every operation rounds
+// once by itself, so that a moment next to the border between two codes gets the
+// same code as from elementary fp32 operations.
+__device__ __forceinline__ void adamw4(const Hyper& h, float* p, const float* grad, float* m, float* v, float* root) {
+  {
+#pragma clang fp contract(off)
+#pragma unroll
+    for (int e = 0; e < kVec; ++e) {
+      const float g = grad[e] * h.grad_scale;
+      m[e] = h.beta1 * m[e] + h.one_minus_beta1 * g;
+      v[e] = h.beta2 * v[e] + h.one_minus_beta2 * (g * g);
+    }
+  }
+  sqrt4(v, root);
+#pragma unroll
+  for (int e = 0; e < kVec; ++e) {
+    const float denom = root[e] * h.inv_root_bias + h.eps;    // never denormal: the host refuses such an eps
+#if defined(__HIP_DEVICE_COMPILE__)
+    const float update = m[e] * __builtin_amdgcn_rcpf(denom);  // one unit in the last place and one rounding
+#else
+    const float update = m[e] / denom;
+#endif
+    p[e] -= h.lr_decay * p[e] + h.step_size * update;   // the two small terms first: 1 - lr * decay would round them away
+  }
+}
 
-// Moments in 32 bits: one wave per U * 256 elements.
-template <class P, class G, class C, int U, bool NT>
-__global__ __launch_bounds__(kWave) void k_adamw(AdamTable t, int count, Hyper h) {
-  const int s = find_segment(t.start, count, blockIdx.x);
-  const size_t n = t.n[s];
-  const size_t base = (size_t)(blockIdx.x - t.start[s]) * (U * kBlock) + (threadIdx.x & (kWave - 1)) * kVec;
+// A tensor may start anywhere; the waves' shares are laid out so that their
+// first moments start at multiples of 256 bytes.  Pieces of flat buffers that
+// start at the same element of each have their other streams aligned with it.
+// The first share then has this many elements before the tensor's start.
+// Without it two waves share the cache lines at every border, and their
+// non-temporal stores go to memory as partial lines.
+__host__ __device__ __forceinline__ uint32_t lead(const void* m) { return (uint32_t)((uintptr_t)m / 4 % 64); }
+
+// Moments in 32 bits: one wave per 256 elements.
+template <class P, class G, class C, bool NT>
+__global__ __launch_bounds__(kWave) void k_adamw(AdamTable args, const void* dev, int count, Hyper h) {
+  const View<AdamEntry> t = view_of(args, dev, count);
+  const int s = find_segment(t, count, blockIdx.x);
   if (!finish_hyper(h)) return;
-  float p[U][kVec], g[U][kVec], m[U][kVec], v[U][kVec];
-#pragma unroll
-  for (int u = 0; u < U; ++u) {
-    const size_t i = base + u * kBlock;
-    load_upto4<P, NT>(t.p[s], i, n, p[u]);
-    load_upto4<G, NT>(t.g[s], i, n, g[u]);
-    load_upto4<F32, NT>(t.m[s], i, n, m[u]);
-    load_upto4<F32, NT>(t.v[s], i, n, v[u]);
-  }
-#pragma unroll
-  for (int u = 0; u < U; ++u) {
-    const size_t i = base + u * kBlock;
-#pragma unroll
-    for (int e = 0; e < kVec; ++e) adamw_element(h, p[u][e], g[u][e], m[u][e], v[u][e]);
-    store_upto4<P, NT>(t.p[s], i, n, p[u]);
-    store_upto4<F32, NT>(t.m[s], i, n, m[u]);
-    store_upto4<F32, NT>(t.v[s], i, n, v[u]);
-    if constexpr (!C::kNone) store_upto4<C, NT>(t.c[s], i, n, p[u]);
-  }
+  const uint32_t before = lead(t.e[s].m), item = blockIdx.x - t.start[s];
+  const ptrdiff_t first = (ptrdiff_t)((size_t)item * kBlock) - before;
+  const size_t end = t.e[s].n - (size_t)first;       // place of the tensor's end
+  const Span span = {item ? 0 : before, at_most(end, kBlock)};
+  const gptr pp = element(t.e[s].p, first, sizeof(typename P::elem));
+  const cgptr gp = element(t.e[s].g, first, sizeof(typename G::elem));
+  const gptr mp = element(t.e[s].m, first, 4);
+  const gptr vp = element(t.e[s].v, first, 4);
+  const gptr cp = C::kNone ? nullptr : element(t.e[s].c, first, 2);
+  const uint32_t i = (threadIdx.x & (kWave - 1)) * kVec;
+  with_bounds(span.lo == 0 && span.hi == kBlock, [&](auto full) {
+    constexpr bool FULL = decltype(full)::value;
+    float p[kVec], g[kVec], m[kVec], v[kVec], root[kVec];
+    load_upto4<P, NT, FULL>(pp, i, span, p);
+    load_upto4<G, NT, FULL>(gp, i, span, g);
+    load_upto4<F32, NT, FULL>(mp, i, span, m);
+    load_upto4<F32, NT, FULL>(vp, i, span, v);
+    adamw4(h, p, g, m, v, root);
+    store_upto4<P, NT, FULL>(pp, i, span, p);
+    store_upto4<F32, NT, FULL>(mp, i, span, m);
+    store_upto4<F32, NT, FULL>(vp, i, span, v);
+    if constexpr (!C::kNone) store_upto4<C, NT, FULL>(cp, i, span, p);
+  });
 }
-
-struct Adam8Table {
-  void* p[kAdam8Segs];
-  const void* g[kAdam8Segs];
-  void* m[kAdam8Segs];         // codes of the first moment
-  void* r[kAdam8Segs];         // codes of the root of the second
-  float* ms[kAdam8Segs];
-  float* rs[kAdam8Segs];
-  void* c[kAdam8Segs];
-  size_t n[kAdam8Segs];
-  uint32_t start[kAdam8Segs];
-};
 
 // Moments in 8 bits: one wave per block.
 template <class P, class G, class C, bool NT>
-__global__ __launch_bounds__(kWave) void k_adamw8(Adam8Table t, int count, Hyper h) {
+__global__ __launch_bounds__(kWave) void k_adamw8(Adam8Table args, const void* dev, int count, Hyper h) {
   if (kHostRun && threadIdx.x) return;
-  const int s = find_segment(t.start, count, blockIdx.x);
-  const size_t n = t.n[s], block = blockIdx.x - t.start[s];
+  const View<Adam8Entry> t = view_of(args, dev, count);
+  const int s = find_segment(t, count, blockIdx.x);
   if (!finish_hyper(h)) return;
-  const float ms = t.ms[s][block], rs = t.rs[s][block];
-  float m[kLaneSlots][kVec], r[kLaneSlots][kVec];
-  uint32_t ma[kLaneSlots], ra[kLaneSlots];
-  each_lane([&](int k, int lane) {
-    const size_t i = block * kBlock + lane * kVec;
-    float p[kVec], g[kVec];
-    load_upto4<P, NT>(t.p[s], i, n, p);
-    load_upto4<G, NT>(t.g[s], i, n, g);
-    decode4(load_codes(t.m[s], i, n), m[k]);
-    decode4(load_codes(t.r[s], i, n), r[k]);
-#pragma unroll
-    for (int e = 0; e < kVec; ++e) {
-      m[k][e] *= ms;
-      const float old = r[k][e] * rs;
-      float v = old * old;
-      r[k][e] = adamw_element(h, p[e], g[e], m[k][e], v);
-    }
-    store_upto4<P, NT>(t.p[s], i, n, p);
-    if constexpr (!C::kNone) store_upto4<C, NT>(t.c[s], i, n, p);
-    ma[k] = amax4(m[k]);
-    ra[k] = amax4(r[k]);
-  });
-  const BlockScale mb = block_scale(wave_max(ma)), rb = block_scale(wave_max(ra));
+  const size_t block = blockIdx.x - t.start[s], first = block * kBlock;
+  const Span span = span_of(first, t.e[s].n, kBlock);
+  const gptr pp = element(t.e[s].p, first, sizeof(typename P::elem));
+  const cgptr gp = element(t.e[s].g, first, sizeof(typename G::elem));
+  const gptr mp = element(t.e[s].m, first, 1);
+  const gptr rp = element(t.e[s].r, first, 1);
+  const gptr cp = C::kNone ? nullptr : element(t.e[s].c, first, 2);
+  PCCL_GLOBAL float* const msp = (PCCL_GLOBAL float*)element(t.e[s].ms, block, 4);
+  PCCL_GLOBAL float* const rsp = (PCCL_GLOBAL float*)element(t.e[s].rs, block, 4);
   const uint32_t key = noise_key(h.seed, h.step);
-  each_lane([&](int k, int lane) {
-    const size_t i = block * kBlock + lane * kVec;
-    float y[kVec], z[kVec];
-#pragma unroll
-    for (int e = 0; e < kVec; ++e) {
-      y[e] = m[k][e] * mb.inv;
-      z[e] = lift_root(r[k][e], r[k][e] * rb.inv);
-    }
-    if (h.stochastic) {
+  with_bounds(span.hi == kBlock, [&](auto full) {
+    constexpr bool FULL = decltype(full)::value;
+    float m[kLaneSlots][kVec], r[kLaneSlots][kVec];
+    uint32_t ma[kLaneSlots], ra[kLaneSlots];
+    const float ms = *msp, rs = *rsp;
+    each_lane([&](int k, int lane) {
+      const uint32_t i = lane * kVec;
+      float p[kVec], g[kVec], v[kVec];
+      load_upto4<P, NT, FULL>(pp, i, span, p);
+      load_upto4<G, NT, FULL>(gp, i, span, g);
+      const uint32_t mc = load_codes<NT, FULL>(mp, i, span), rc = load_codes<NT, FULL>(rp, i, span);
+      decode4(mc, m[k]);
+      decode4(rc, r[k]);
 #pragma unroll
       for (int e = 0; e < kVec; ++e) {
-        const uint32_t bits = noise(key, i + e);
-        y[e] = round_stochastic(y[e], bits & 0xffffu);
-        z[e] = round_stochastic(z[e], bits >> 16);
+        m[k][e] *= ms;
+        r[k][e] *= rs;
+        v[e] = r[k][e] * r[k][e];
       }
-    }
-    store_codes(t.m[s], i, n, encode4(y));
-    store_codes(t.r[s], i, n, encode4(z));
-    if (lane == 0) { t.ms[s][block] = mb.scale; t.rs[s][block] = rb.scale; }
+      adamw4(h, p, g, m[k], v, r[k]);
+      store_upto4<P, NT, FULL>(pp, i, span, p);
+      if constexpr (!C::kNone) store_upto4<C, NT, FULL>(cp, i, span, p);
+      ma[k] = amax4(m[k]);
+      ra[k] = amax4(r[k]);
+    });
+    const BlockScale mb = block_scale(wave_max(ma)), rb = block_scale(wave_max(ra));
+    each_lane([&](int k, int lane) {
+      const uint32_t i = lane * kVec;
+      float y[kVec], z[kVec];
+      uint32_t yc, zc;
+#pragma unroll
+      for (int e = 0; e < kVec; ++e) {
+        y[e] = m[k][e] * mb.inv;
+        z[e] = lift_root(r[k][e], r[k][e] * rb.inv);
+      }
+      if (h.stochastic) {
+        uint32_t yb[kVec], zb[kVec];
+#pragma unroll
+        for (int e = 0; e < kVec; ++e) {
+          const uint32_t bits = noise(key, first, i + e);
+          yb[e] = bits << 16;
+          zb[e] = bits & 0xffff0000u;
+          y[e] = clamp_code(y[e]);
+        }
+        yc = encode4_stochastic(y, yb);
+        zc = encode4_stochastic(z, zb);
+      } else {
+        yc = encode4(y);
+        zc = encode4(z);
+      }
+      store_codes<NT, FULL>(mp, i, span, yc);
+      store_codes<NT, FULL>(rp, i, span, zc);
+      if (lane == 0) { *msp = mb.scale; *rsp = rb.scale; }
+    });
   });
 }
 
 // ---------------------------------------------------------------------------
 // 8-bit blocks
 // ---------------------------------------------------------------------------
-struct BlocksTable {
-  void* codes[kBlockSegs];
-  float* scales[kBlockSegs];
-  void* x[kBlockSegs];
-  size_t n[kBlockSegs];
-  uint32_t start[kBlockSegs];
-};
-
-template <class T, bool NT>
-__global__ __launch_bounds__(kWave) void k_quantize(BlocksTable t, int count, int root) {
+// One wave per U blocks, whose loads are all in flight before the first is used.
+template <class T, int U, bool NT>
+__global__ __launch_bounds__(kWave) void k_quantize(BlocksTable args, int count, int root) {
   if (kHostRun && threadIdx.x) return;
-  const int s = find_segment(t.start, count, blockIdx.x);
-  const size_t n = t.n[s], block = blockIdx.x - t.start[s];
-  float x[kLaneSlots][kVec];
-  uint32_t a[kLaneSlots];
-  each_lane([&](int k, int lane) {
-    load_upto4<T, NT>(t.x[s], block * kBlock + lane * kVec, n, x[k]);
-    if (root)
-      for (int e = 0; e < kVec; ++e) x[k][e] = sqrtf(x[k][e]);
-    a[k] = amax4(x[k]);
-  });
-  const BlockScale b = block_scale(wave_max(a));
-  each_lane([&](int k, int lane) {
-    float y[kVec];
-    for (int e = 0; e < kVec; ++e) {
-      y[e] = x[k][e] * b.inv;
-      if (root) y[e] = lift_root(x[k][e], y[e]);
+  const View<BlocksEntry> t = view_of(args, nullptr, count);
+  const int s = find_segment(t, count, blockIdx.x);
+  const size_t block = (size_t)(blockIdx.x - t.start[s]) * U, first = block * kBlock;
+  const Span span = span_of(first, t.e[s].n, U * kBlock);
+  const gptr codes = element(t.e[s].codes, first, 1);
+  const cgptr xp = element(t.e[s].x, first, sizeof(typename T::elem));
+  PCCL_GLOBAL float* const scales = (PCCL_GLOBAL float*)element(t.e[s].scales, block, 4);
+  with_bounds(span.hi == U * kBlock, [&](auto full) {
+    constexpr bool FULL = decltype(full)::value;
+    float x[kLaneSlots][U][kVec];
+    each_lane([&](int k, int lane) {
+#pragma unroll
+      for (int u = 0; u < U; ++u) load_upto4<T, NT, FULL>(xp, u * kBlock + lane * kVec, span, x[k][u]);
+    });
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      if (!FULL && u * kBlock >= span.hi) break;
+      uint32_t a[kLaneSlots];
+      each_lane([&](int k, int) {
+        if (root)
+          for (int e = 0; e < kVec; ++e) x[k][u][e] = sqrtf(x[k][u][e]);
+        a[k] = amax4(x[k][u]);
+      });
+      const BlockScale b = block_scale(wave_max(a));
+      each_lane([&](int k, int lane) {
+        float y[kVec];
+#pragma unroll
+        for (int e = 0; e < kVec; ++e) {
+          y[e] = x[k][u][e] * b.inv;
+          if (root) y[e] = lift_root(x[k][u][e], y[e]);
+        }
+        store_codes<NT, FULL>(codes, u * kBlock + lane * kVec, span, encode4(y));
+        if (lane == 0) scales[u] = b.scale;
+      });
     }
-    store_codes(t.codes[s], block * kBlock + lane * kVec, n, encode4(y));
-    if (lane == 0) t.scales[s][block] = b.scale;
   });
 }
 
-template <class T, bool NT>
-__global__ __launch_bounds__(kWave) void k_dequantize(BlocksTable t, int count, int root) {
-  const int s = find_segment(t.start, count, blockIdx.x);
-  const size_t n = t.n[s], block = blockIdx.x - t.start[s];
-  const size_t i = block * kBlock + (threadIdx.x & (kWave - 1)) * kVec;
-  const float scale = t.scales[s][block];
-  float x[kVec];
-  decode4(load_codes(t.codes[s], i, n), x);
-  for (int e = 0; e < kVec; ++e) {
-    x[e] *= scale;
-    if (root) x[e] *= x[e];
-  }
-  store_upto4<T, NT>(t.x[s], i, n, x);
+template <class T, int U, bool NT>
+__global__ __launch_bounds__(kWave) void k_dequantize(BlocksTable args, int count, int root) {
+  const View<BlocksEntry> t = view_of(args, nullptr, count);
+  const int s = find_segment(t, count, blockIdx.x);
+  const size_t block = (size_t)(blockIdx.x - t.start[s]) * U, first = block * kBlock;
+  const Span span = span_of(first, t.e[s].n, U * kBlock);
+  const cgptr codes = element(t.e[s].codes, first, 1);
+  const gptr xp = element(t.e[s].x, first, sizeof(typename T::elem));
+  const PCCL_GLOBAL float* const scales = (const PCCL_GLOBAL float*)element(t.e[s].scales, block, 4);
+  const uint32_t lane4 = (threadIdx.x & (kWave - 1)) * kVec;
+  with_bounds(span.hi == U * kBlock, [&](auto full) {
+    constexpr bool FULL = decltype(full)::value;
+    uint32_t w[U];
+    float scale[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      w[u] = load_codes<NT, FULL>(codes, u * kBlock + lane4, span);
+      scale[u] = FULL || u * kBlock < span.hi ? scales[u] : 0.0f;
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      float x[kVec];
+      decode4(w[u], x);
+#pragma unroll
+      for (int e = 0; e < kVec; ++e) {
+        x[e] *= scale[u];
+        if (root) x[e] *= x[e];
+      }
+      store_upto4<T, NT, FULL>(xp, u * kBlock + lane4, span, x);
+    }
+  });
 }
 
 // ---------------------------------------------------------------------------
 // gradient norm
 // ---------------------------------------------------------------------------
-constexpr int kNormThreads = 256;
-constexpr int kNormUnroll = 4;
-constexpr int kNormTile = kNormThreads * kVec * kNormUnroll;     // elements of a work item
-
-struct NormTable {
-  const void* x[kNormSegs];
-  size_t n[kNormSegs];
-  uint32_t start[kNormSegs];
-};
+constexpr int kNormUnroll = 8;                              // 16-byte vectors of a lane in one work item
+constexpr size_t kNormBytes = (size_t)kWave * 16 * kNormUnroll;   // a work item: what one wave reads at once
 
 // Sum over the threads of a workgroup, in a fixed order; valid in thread 0.
 // `part`: the thread's own value on the device, all threads' on the host.
@@ -543,47 +759,97 @@ __device__ __forceinline__ double group_sum(const double* part) {
 #endif
 }
 
-// One partial sum per workgroup, which walks the work items gridDim.x apart.
+// The elements of a 16-byte vector
+template <class T> struct Vec16 {
+  static constexpr int kCount = 16 / sizeof(typename T::elem);
+  typedef typename T::elem elems __attribute__((ext_vector_type(kCount)));
+  typedef float floats __attribute__((ext_vector_type(kCount)));
+};
+
+// Sum of the squares of a vector.  In fp32, as a tree of at most four roundings,
+// where the result says that nothing overflowed and that what underflowed does
+// not count; else (zeros, too) in 64 bits, where no square of an fp32 number is
+// out of range.  All in 64 bits is bound by arithmetic: see k_sum_squares.
+template <int N, class V> __device__ __forceinline__ double sum_squares(const V& x) {
+  float t[N / 2];
+#pragma unroll
+  for (int e = 0; e < N / 2; ++e) t[e] = x[2 * e] * x[2 * e] + x[2 * e + 1] * x[2 * e + 1];
+#pragma unroll
+  for (int w = N / 4; w; w /= 2)
+#pragma unroll
+    for (int e = 0; e < w; ++e) t[e] += t[e + w];
+  if (t[0] >= 0x1p-100f && t[0] <= 0x1p126f) return (double)t[0];
+  double sum = 0;
+#pragma unroll
+  for (int e = 0; e < N; ++e) sum += (double)x[e] * (double)x[e];
+  return sum;
+}
+
+// One partial sum per workgroup of T threads; every wave walks the work items
+// that lie as many apart as the grid has waves.
 // FINAL: the only workgroup of the whole norm; it writes the result itself.
-template <class T, bool NT, bool FINAL>
-__global__ __launch_bounds__(kNormThreads) void k_sum_squares(NormTable t, int count, uint32_t items, double* part, float* out) {
+template <class E, int T, bool NT, bool FINAL>
+__global__ __launch_bounds__(T) void k_sum_squares(NormTable args, int count, uint32_t items, double* part, float* out) {
   if (kHostRun && threadIdx.x) return;
-  constexpr int kSlots = kHostRun ? kNormThreads : 1;
+  typedef Vec16<E> V;
+  typedef typename E::elem elem;
+  constexpr uint32_t kElems = kNormBytes / sizeof(elem);
+  constexpr int kSlots = kHostRun ? T : 1;
+  const View<NormEntry> t = view_of(args, nullptr, count);
   double sum[kSlots];
   for (int k = 0; k < kSlots; ++k) {
-    const int thread = kHostRun ? k : (int)threadIdx.x;
+    const uint32_t thread = kHostRun ? (uint32_t)k : threadIdx.x;
+    const uint32_t lane = thread & (kWave - 1);
     double acc = 0;
-    for (uint32_t item = blockIdx.x; item < items; item += gridDim.x) {
-      const int s = find_segment(t.start, count, item);
-      const size_t n = t.n[s];
-      const size_t base = (size_t)(item - t.start[s]) * kNormTile + (size_t)thread * kVec;
-      float x[kNormUnroll][kVec];
+    for (uint32_t item = blockIdx.x * (T / kWave) + wave_uniform(thread / kWave); item < items; item += gridDim.x * (T / kWave)) {
+      const int s = find_segment(t, count, item);
+      const size_t first = (size_t)(item - t.start[s]) * kElems;
+      const uint32_t left = span_of(first, t.e[s].n, kElems).hi;
+      const PCCL_GLOBAL elem* x = (const PCCL_GLOBAL elem*)element(t.e[s].x, first, sizeof(elem));
+      if (left == kElems) {
+        u32x4a w[kNormUnroll];
 #pragma unroll
-      for (int u = 0; u < kNormUnroll; ++u) load_upto4<T, NT>(t.x[s], base + u * (kNormThreads * kVec), n, x[u]);
+        for (int u = 0; u < kNormUnroll; ++u) w[u] = load16<NT>((cgptr)x + (u * kWave + lane) * 16u);
 #pragma unroll
-      for (int u = 0; u < kNormUnroll; ++u)
-#pragma unroll
-        for (int e = 0; e < kVec; ++e) acc += (double)x[u][e] * (double)x[u][e];
+        for (int u = 0; u < kNormUnroll; ++u) {
+          typename V::elems e;
+          __builtin_memcpy(&e, &w[u], 16);
+          acc += sum_squares<V::kCount>(__builtin_convertvector(e, typename V::floats));
+        }
+      } else {
+        for (int u = 0; u < kNormUnroll; ++u) {
+          const uint32_t i = (u * kWave + lane) * V::kCount;
+          if (i + V::kCount <= left) {
+            const u32x4a w = load16<false>((cgptr)x + i * (uint32_t)sizeof(elem));
+            typename V::elems e;
+            __builtin_memcpy(&e, &w, 16);
+            acc += sum_squares<V::kCount>(__builtin_convertvector(e, typename V::floats));
+          } else {
+            for (uint32_t j = i; j < left && j < i + V::kCount; ++j) acc += (double)(float)x[j] * (double)(float)x[j];
+          }
+        }
+      }
     }
     sum[k] = acc;
   }
-  const double total = group_sum<kNormThreads>(sum);
+  const double total = group_sum<T>(sum);
   if (threadIdx.x == 0) {
     if constexpr (FINAL) out[0] = (float)sqrt(total);
     else part[blockIdx.x] = total;
   }
 }
 
-__global__ __launch_bounds__(kNormThreads) void k_norm_join(const double* part, uint32_t count, float* out) {
+// One wave adds the partial sums up.
+__global__ __launch_bounds__(kWave) void k_norm_join(const double* part, uint32_t count, float* out) {
   if (kHostRun && threadIdx.x) return;
-  constexpr int kSlots = kHostRun ? kNormThreads : 1;
-  double sum[kSlots];
-  for (int k = 0; k < kSlots; ++k) {
+  double sum[kLaneSlots];
+  each_lane([&](int k, int lane) {
     double acc = 0;
-    for (uint32_t i = kHostRun ? k : threadIdx.x; i < count; i += kNormThreads) acc += part[i];
+#pragma unroll 4
+    for (uint32_t i = lane; i < count; i += kWave) acc += part[i];
     sum[k] = acc;
-  }
-  const double total = group_sum<kNormThreads>(sum);
+  });
+  const double total = group_sum<kWave>(sum);
   if (threadIdx.x == 0) out[0] = (float)sqrt(total);
 }
 

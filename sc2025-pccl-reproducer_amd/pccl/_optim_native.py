@@ -37,7 +37,9 @@ SIGNATURES = {
     "pccl_optim_plan_free": (None, [_vp]),
     "pccl_optim_plan_adamw": (_int, [_vpp, _vpp, _vpp, _vpp, _vpp, _vpp, _szp, _intp, _intp, _intp, _int]),
     "pccl_optim_plan_adamw8": (_int, [_vpp, _vpp, _vpp, _vpp, _vpp, _vpp, _vpp, _vpp, _szp, _intp, _intp, _intp, _int]),
-    "pccl_optim_run_adamw": (_int, [_vp, _vpp, ctypes.POINTER(Step), _vp]),
+    "pccl_optim_table_bytes": (_sz, [_vp]),
+    "pccl_optim_table_fill": (_int, [_vp, _vp, _sz]),
+    "pccl_optim_run_adamw": (_int, [_vp, _vpp, _vp, ctypes.POINTER(Step), _vp]),
     "pccl_optim_plan_norm": (_int, [_vpp, _vpp, _szp, _intp, _int]),
     "pccl_optim_norm_work": (_sz, [_vp]),
     "pccl_optim_run_norm": (_int, [_vp, _vp, _vp, _sz, _vp]),
@@ -118,8 +120,14 @@ class OptimLib:
                           _size_table(n), _int_table(dtype), len(n), 1 if root else 0)
 
     # -- runs ----------------------------------------------------------------
-    def run_adamw(self, plan: Plan, step: Step, grads=None, stream=0):
-        self.check(self.run_adamw_fn(plan.handle, _ptr_table(grads), ctypes.byref(step), stream))
+    def table_bytes(self, plan: Plan) -> int:
+        return self._lib.pccl_optim_table_bytes(plan.handle)
+
+    def table_fill(self, plan: Plan, host: int, nbytes: int):
+        self.check(self._lib.pccl_optim_table_fill(plan.handle, host, nbytes))
+
+    def run_adamw(self, plan: Plan, step: Step, grads=None, table=None, stream=0):
+        self.check(self.run_adamw_fn(plan.handle, _ptr_table(grads), table, ctypes.byref(step), stream))
 
     def norm_work(self, plan: Plan) -> int:
         return self._lib.pccl_optim_norm_work(plan.handle)

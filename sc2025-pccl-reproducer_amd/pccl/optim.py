@@ -113,10 +113,14 @@ def _scalar(what, name, t, dtype, device):
 
 def _on(device, fn, *args):
     """fn(*args, stream) on the current stream of `device`, whatever the current device is."""
-    if device is None or device.type != "cuda" or device.index == torch.cuda.current_device():
+    if device is None or device.type != "cuda" or device.index == kernels._current_device():
         return fn(*args, kernels.stream_handle())
     with torch.cuda.device(device):
         return fn(*args, kernels.stream_handle())
+
+
+def _capturing(device):
+    return device is not None and device.type == "cuda" and torch.cuda.is_current_stream_capturing()
 
 
 def _hold(*lists):
@@ -128,7 +132,8 @@ def _hold(*lists):
 class _Plan:
     def __init__(self, lib, native, device, keep, written=()):
         self._lib, self._native, self._device, self._keep = lib, native, device, keep
-        self._written = list(written)      # their version counters are raised, as an in-place torch operation would
+        # what to raise the version counters of, as an in-place torch operation would: views share their base's
+        self._written = list({id(b): b for b in (t if t._base is None else t._base for t in written)}.values())
 
     def _done(self, rc):
         if rc:
@@ -195,7 +200,29 @@ class AdamWPlan(_Plan):
                                        f"({dtype}, {tuple(shape)}), got {g.dtype}, {tuple(g.shape)}")
                 _check_device(self._what, f"grads[{i}]", g, self._device)
             table = _optim_native._ptr_table([g.data_ptr() for g in grads])
-        self._done(_on(self._device, self._lib.run_adamw_fn, self._native.handle, table, s))
+        self._done(_on(self._device, self._run, table, s))
+
+    def _run(self, grads, step, stream):
+        table = None
+        if self._table is not None and grads is None and stream == self._table_stream and not _capturing(self._device):
+            table = self._table.data_ptr()
+        return self._lib.run_adamw_fn(self._native.handle, grads, table, step, stream)
+
+    def _make_table(self):
+        """The addresses of more tensors than one launch takes in its arguments, in
+        device memory.  It is written, read and freed on ONE stream, the one the
+        plan is made on; calls on other streams and captured calls (a graph may
+        outlive the plan) pass the addresses in arguments, in a few launches."""
+        self._table = None
+        size = self._lib.table_bytes(self._native)
+        if not size or _capturing(self._device):
+            return
+        host = torch.empty(size, dtype=torch.uint8)
+        self._lib.table_fill(self._native, host.data_ptr(), size)
+
+        def put(stream):
+            self._table, self._table_stream = host.to(self._device), stream
+        _on(self._device, put)
 
 
 def _plan_adamw(what, eight, params, grads, first, second, scales, copies, lr, betas, eps, weight_decay):
@@ -232,6 +259,7 @@ def _plan_adamw(what, eight, params, grads, first, second, scales, copies, lr, b
     plan = AdamWPlan(lib, native, device, _hold(params, grads, first, second, copies, *(scales or ())), written)
     plan._what = what
     plan._prepare(eight, grads, lr, betas, eps, weight_decay)
+    plan._make_table()
     return plan
 
 

@@ -75,7 +75,8 @@ def adamw(p, g, m, v, step, *, lr, betas, eps, weight_decay, grad_scale=1.0, nor
     ed = er / bias2 + 3 * U * den + TINY
     with np.errstate(divide="ignore", invalid="ignore"):
         upd = mn / den
-        eu = np.where(den > ed, (em + np.abs(upd) * ed) / np.maximum(den - ed, TINY) + U * np.abs(upd) + TINY, np.inf)
+        # m * (1 / den): the reciprocal instruction is good to one unit in the last place (2 U), and one rounding
+        eu = np.where(den > ed, (em + np.abs(upd) * ed) / np.maximum(den - ed, TINY) + 3.1 * U * np.abs(upd) + TINY, np.inf)
         size = lr / bias1
         change = lr * weight_decay * p + size * upd
         ec = 3 * U * (np.abs(lr * weight_decay * p) + np.abs(size * upd)) + size * eu + 3 * TINY

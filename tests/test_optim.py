@@ -277,6 +277,29 @@ def test_more_tensors_than_one_launch_holds_and_mixed_types(where, eight):
             check_adamw(s, old[i], 4, f"tensor {i}", **HYPER)
 
 
+@pytest.mark.parametrize("count", [57, 64, 65, 300, 4200])
+@pytest.mark.parametrize("eight", [False, True])
+def test_many_tensors_of_one_type(where, count, eight):
+    """Addresses in kernel arguments, in a table in device memory (once for up to 4096), and with other gradients."""
+    from pccl import optim
+    gen = np.random.default_rng(count)
+    sizes = [int(x) for x in gen.choice([0, 1, 3, 255, 256, 257, 300] if count < 1000 else [0, 1, 2, 5], count)]
+    s = make(sizes, where.device, g="bf16", c="f16", gap=1, seed=15, eight=eight)
+    other = make(sizes, where.device, g="bf16", gap=2, seed=16)
+    keys = ("p", "g", "m", "r", "ms", "rs") if eight else ("p", "g", "m", "v")
+    plan = (optim.plan_adamw8 if eight else optim.plan_adamw)(*(s[k].list for k in keys), copies=s["c"].list, **HYPER)
+    assert (plan._table is not None) == (sum(n > 0 for n in sizes) > (56 if eight else 64))
+    check, read = (check_adamw8, values8) if eight else (check_adamw, lambda s: values(s, "pgmv"))
+    old = read(s)
+    plan(3)
+    where.sync()
+    check(s, old, 3, "own gradients", **HYPER)
+    old = dict(read(s), g=values(other, "g")["g"])
+    plan(4, grads=other["g"].list)
+    where.sync()
+    check(s, old, 4, "other gradients", **HYPER)
+
+
 def test_plan_takes_other_gradients(where):
     from pccl import optim
     s = make([3, 900], where.device, g="bf16", seed=10)
@@ -903,7 +926,8 @@ def test_c_entries_refuse_with_a_code_and_a_message():
     assert raw.pccl_optim_plan_norm(ctypes.byref(h), None, None, None, 1) == -1 and not h
     assert raw.pccl_optim_run_norm(None, None, None, 0, None) == -1
     assert raw.pccl_optim_run_blocks(None, None) == -1
-    assert raw.pccl_optim_run_adamw(None, None, None, None) == -1
+    assert raw.pccl_optim_run_adamw(None, None, None, None, None) == -1
+    assert raw.pccl_optim_table_fill(None, None, 0) == -1 and raw.pccl_optim_table_bytes(None) == 0
     assert raw.pccl_optim_norm_work(None) == 0
     raw.pccl_optim_plan_free(None)
     norm = lib.plan_norm([64], [1 << 20], [0])
@@ -919,6 +943,16 @@ def test_c_entries_refuse_with_a_code_and_a_message():
         lib.run_adamw(step, s, [0])
     with pytest.raises(E, match="not aligned"):
         lib.run_adamw(step, s, [66])
+    with pytest.raises(E, match="has no table"):
+        lib.run_adamw(step, s, None, 64)
+    many = lib.plan_adamw(*[[(1 + k) << 20 | i << 6 for i in range(65)] for k in range(4)], None, [4] * 65, [0] * 65, [0] * 65, None)
+    assert lib.table_bytes(many) >= 65 * 52
+    with pytest.raises(E, match="bytes, got"):
+        lib.table_fill(many, 64, 65 * 52 - 1)
+    with pytest.raises(E, match="not aligned to 64"):
+        lib.run_adamw(many, s, None, 32)
+    with pytest.raises(E, match="another operator"):
+        lib.table_fill(norm, 64, 1 << 20)
 
 
 def test_header_lists_what_the_binding_and_the_library_have():
