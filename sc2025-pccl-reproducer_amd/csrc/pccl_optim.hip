@@ -53,16 +53,21 @@ int launch_status(const char* what) {
   return PCCL_HIP_OK;
 }
 
-// Tensors that together exceed the Infinity Cache (256 MiB) and the L2s stream:
-// their accesses carry the non-temporal hint.
-constexpr size_t kStreamFrom = (size_t)288 << 20;
+// Plans whose tensors take this much memory together get the non-temporal hint on
+// all accesses.  On data that has left the caches it is better at any size
+// (AdamW over 29 / 117 / 235 MB: 9.8 / 25 / 43 us against 12.2 / 28 / 50; norm of
+// 67 MB 17.5 against 29); on data that is still in the 256 MiB Infinity Cache it
+// is worse (AdamW over 117 MB called on three such sets in turn 21.6 against
+// 19.0).  A third of the cache is where calls in turn no longer find their data.
+constexpr size_t kStreamFrom = (size_t)96 << 20;
 
 // Work items of one launch.  The grid is counted in threads, in 32 bits.
 constexpr size_t kMaxItems = ((size_t)1 << 26) - 1;
 
-// Work of one wave (see the kernels): blocks of 256 elements for k_quantize, by the size of the source's element, and
-// for k_dequantize
-constexpr int kQuantizeWide = 4, kQuantizeNarrow = 8, kDequantizeBlocks = 4;
+// Blocks of one wave: 4 KiB of what k_quantize reads (128 Mi elements, us at 1 / 2 / 4 / 8 blocks: bf16 135 101 72
+// 67), 2 KiB of what k_dequantize writes (bf16 118 82 64 66; fp32 139 107 121 122)
+template <class T> constexpr int kQuantizeBlocks = 4096 / (kBlock * sizeof(typename T::elem));
+template <class T> constexpr int kDequantizeBlocks = 2048 / (kBlock * sizeof(typename T::elem));
 
 constexpr int kNormThreads = 1024;        // threads of a workgroup of the norm
 constexpr uint32_t kNormGroups = 256;     // workgroups, and partial sums, of one launch
@@ -328,7 +333,7 @@ int make_adamw(pccl_optim_plan& plan, Checker& check, void* const* params, const
     plan.f.push_back(eight ? vs[i] : nullptr);
     plan.gtype.push_back(gt[i]);
   }
-  return make_batches(plan, pt, gt, ctype.data(), [&](int i) { return blocks_of(plan.n[i] + (eight ? 0 : lead(m[i]))); },
+  return make_batches(plan, pt, gt, ctype.data(), [&](int i) { return eight ? items_for(plan.n[i], (esize_of(pt[i]) == 4 ? kAdam8Blocks<F32> : kAdam8Blocks<BF16>) * kBlock) : blocks_of(plan.n[i] + lead(m[i])); },
                       kTableMax, check.what);
 }
 
@@ -424,8 +429,8 @@ struct AdamLaunch {
       });
     else
       each_launch<Adam8Table>(plan, b, grads, dev, [&](const Adam8Table& t, const Share& s) {
-        if (plan.stream) PCCL_LAUNCH((k_adamw8<P, G, C, true>), dim3(s.items), dim3(kWave), 0, stream, t, s.dev, s.count, h);
-        else PCCL_LAUNCH((k_adamw8<P, G, C, false>), dim3(s.items), dim3(kWave), 0, stream, t, s.dev, s.count, h);
+        if (plan.stream) PCCL_LAUNCH((k_adamw8<P, G, C, kAdam8Blocks<P>, true>), dim3(s.items), dim3(kWave), 0, stream, t, s.dev, s.count, h);
+        else PCCL_LAUNCH((k_adamw8<P, G, C, kAdam8Blocks<P>, false>), dim3(s.items), dim3(kWave), 0, stream, t, s.dev, s.count, h);
       });
   }
 };
@@ -442,14 +447,14 @@ struct BlocksLaunch {
   const Batch& b;
   hipStream_t stream;
   template <class T> void operator()() const {
-    constexpr int U = sizeof(typename T::elem) == 4 ? kQuantizeWide : kQuantizeNarrow;
+    constexpr int Q = kQuantizeBlocks<T>, D = kDequantizeBlocks<T>;
     each_launch<BlocksTable>(plan, b, nullptr, nullptr, [&](const BlocksTable& t, const Share& s) {
       if (plan.kind == kQuantize) {
-        if (plan.stream) PCCL_LAUNCH((k_quantize<T, U, true>), dim3(s.items), dim3(kWave), 0, stream, t, s.count, plan.root);
-        else PCCL_LAUNCH((k_quantize<T, U, false>), dim3(s.items), dim3(kWave), 0, stream, t, s.count, plan.root);
+        if (plan.stream) PCCL_LAUNCH((k_quantize<T, Q, true>), dim3(s.items), dim3(kWave), 0, stream, t, s.count, plan.root);
+        else PCCL_LAUNCH((k_quantize<T, Q, false>), dim3(s.items), dim3(kWave), 0, stream, t, s.count, plan.root);
       } else {
-        if (plan.stream) PCCL_LAUNCH((k_dequantize<T, kDequantizeBlocks, true>), dim3(s.items), dim3(kWave), 0, stream, t, s.count, plan.root);
-        else PCCL_LAUNCH((k_dequantize<T, kDequantizeBlocks, false>), dim3(s.items), dim3(kWave), 0, stream, t, s.count, plan.root);
+        if (plan.stream) PCCL_LAUNCH((k_dequantize<T, D, true>), dim3(s.items), dim3(kWave), 0, stream, t, s.count, plan.root);
+        else PCCL_LAUNCH((k_dequantize<T, D, false>), dim3(s.items), dim3(kWave), 0, stream, t, s.count, plan.root);
       }
     });
   }
@@ -514,9 +519,7 @@ int plan_blocks(pccl_optim_plan** out, Kind kind, const void* const* codes, cons
       plan.b.push_back((void*)scales[i]);
       plan.c.push_back((void*)x[i]);
     }
-    auto items = [&](int i) {
-      return items_for(n[i], (size_t)kBlock * (!q ? kDequantizeBlocks : esize_of(dtype[i]) == 4 ? kQuantizeWide : kQuantizeNarrow));
-    };
+    auto items = [&](int i) { return items_for(n[i], (q ? 4096 : 2048) / esize_of(dtype[i])); };
     return make_batches(plan, dtype, nullptr, nullptr, items, BlocksTable::kInline, what);
   });
 }

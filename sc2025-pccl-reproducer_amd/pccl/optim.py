@@ -54,17 +54,21 @@ def empty_blocks(tensor: torch.Tensor) -> Tuple[torch.Tensor, torch.Tensor]:
 def _check_list(what, name, tensors, like=None, dtype=None):
     """A list of tensors as long as `like`, on one GPU, each with the size of its partner."""
     tensors = list(tensors)
-    if like is not None and len(tensors) != len(like):
+    if like is None:
+        like = tensors
+    if len(tensors) != len(like):
         raise ValueError(f"{what}: need one {name} tensor per entry of the first list ({len(like)}), got {len(tensors)}")
-    for i, t in enumerate(tensors):
-        kernels.check_device_tensor(t, f"{name}[{i}]")
+    device = None
+    for i, (t, p) in enumerate(zip(tensors, like)):
+        kernels.check_device_tensor(t, name)
         if dtype is not None and t.dtype != dtype:
             raise RuntimeError(f"{what}: {name}[{i}] must be of type {dtype}, got {t.dtype}")
-        if like is not None:
-            p = like[i]
-            if t.numel() != p.numel() or (t.shape != p.shape and t.dim() > 1 and p.dim() > 1):
-                raise RuntimeError(f"{what}: {name}[{i}] has shape {tuple(t.shape)}, its partner {tuple(p.shape)}")
-            _check_device(what, f"{name}[{i}]", t, p.device)
+        if t.shape != p.shape and (t.numel() != p.numel() or (t.dim() > 1 and p.dim() > 1)):
+            raise RuntimeError(f"{what}: {name}[{i}] has shape {tuple(t.shape)}, its partner {tuple(p.shape)}")
+        if device is None:
+            device = like[0].device
+        if t.device != device:
+            _check_device(what, f"{name}[{i}]", t, device)
     return tensors
 
 
@@ -86,19 +90,14 @@ def _check_scales(what, name, scales, codes):
 
 
 def _type_codes(what, name, tensors):
-    out = []
+    codes = {}
     for i, t in enumerate(tensors):
-        try:
-            out.append(kernels.dtype_code(t.dtype))
-        except RuntimeError:
-            raise RuntimeError(f"{what}: {name}[{i}] must be float32, bfloat16 or float16, got {t.dtype}") from None
-    return out
-
-
-def _one_device(what, tensors):
-    for t in tensors[1:]:
-        _check_device(what, "a tensor", t, tensors[0].device)
-    return tensors[0].device if tensors else None
+        if t.dtype not in codes:
+            try:
+                codes[t.dtype] = kernels.dtype_code(t.dtype)
+            except RuntimeError:
+                raise RuntimeError(f"{what}: {name}[{i}] must be float32, bfloat16 or float16, got {t.dtype}") from None
+    return [codes[t.dtype] for t in tensors]
 
 
 def _scalar(what, name, t, dtype, device):
@@ -111,16 +110,8 @@ def _scalar(what, name, t, dtype, device):
     return t.data_ptr()
 
 
-def _on(device, fn, *args):
-    """fn(*args, stream) on the current stream of `device`, whatever the current device is."""
-    if device is None or device.type != "cuda" or device.index == kernels._current_device():
-        return fn(*args, kernels.stream_handle())
-    with torch.cuda.device(device):
-        return fn(*args, kernels.stream_handle())
-
-
-def _capturing(device):
-    return device is not None and device.type == "cuda" and torch.cuda.is_current_stream_capturing()
+def _capturing(index):
+    return index is not None and torch.cuda.is_current_stream_capturing()
 
 
 def _hold(*lists):
@@ -131,11 +122,20 @@ def _hold(*lists):
 
 class _Plan:
     def __init__(self, lib, native, device, keep, written=()):
-        self._lib, self._native, self._device, self._keep = lib, native, device, keep
+        self._lib, self._native, self._handle, self._device, self._keep = lib, native, native.handle, device, keep
+        self._index = device.index if device is not None and device.type == "cuda" else None
         # what to raise the version counters of, as an in-place torch operation would: views share their base's
         self._written = list({id(b): b for b in (t if t._base is None else t._base for t in written)}.values())
 
-    def _done(self, rc):
+    def _on_device(self, fn, *args):
+        """fn(*args, stream) on the current stream of the tensors' device, whatever the current device is."""
+        if self._index is None or self._index == kernels._current_device():
+            return fn(*args, kernels.stream_handle())
+        with torch.cuda.device(self._index):
+            return fn(*args, kernels.stream_handle())
+
+    def _run(self, fn, *args):
+        rc = self._on_device(fn, *args)
         if rc:
             self._lib.check(rc)
         if self._written:
@@ -149,33 +149,53 @@ class _Plan:
 class AdamWPlan(_Plan):
     """One AdamW step over fixed tensors; made by plan_adamw and plan_adamw8."""
 
-    _what = "adamw"
-
-    def _prepare(self, eight, grads, lr, betas, eps, weight_decay):
-        self._eight = eight
-        # (length, type) of each gradient, for calls that bring others
-        self._like = [(g.numel(), g.shape, g.dtype) for g in grads]
+    def _prepare(self, what, grads, lr, betas, eps, weight_decay):
+        self._what = what
+        self._like = [(g.numel(), g.shape, g.dtype) for g in grads]      # for calls that bring other gradients
         self._base = Step(beta1=betas[0], beta2=betas[1], eps=eps, weight_decay=weight_decay, grad_scale=1.0)
-        self._lr = lr
-        self._step(1, lr)
+        self._set_lr(self._base, lr)
+        self._keep.append(lr)
+        self._make_table()
 
-    def _step(self, step, lr):
-        s = Step.from_buffer_copy(self._base)
-        if isinstance(step, torch.Tensor):
-            s.step_dev = _scalar(self._what, "step", step, torch.int64, self._device)
-        else:
-            s.step = step
+    def _set_lr(self, s, lr):
         if isinstance(lr, torch.Tensor):
             s.lr_dev = _scalar(self._what, "lr", lr, torch.float32, self._device)
         else:
-            s.lr = lr
-        return s
+            s.lr_dev, s.lr = None, lr
+
+    def _make_table(self):
+        """The addresses of more tensors than one launch takes in its arguments, in
+        device memory.  It is written, read and freed on ONE stream, the one the
+        plan is made on; calls on other streams and captured calls (a graph may
+        outlive the plan) pass the addresses in arguments, in a few launches."""
+        self._table = self._table_stream = None
+        size = self._lib.table_bytes(self._native)
+        if not size or _capturing(self._index):
+            return
+        host = torch.empty(size, dtype=torch.uint8)
+        self._lib.table_fill(self._native, host.data_ptr(), size)
+
+        def put(stream):
+            self._table, self._table_stream = host.to(self._device), stream
+        self._on_device(put)
+
+    def _step(self, grads, s, stream):
+        table = None
+        if self._table is not None and grads is None and stream == self._table_stream and not _capturing(self._index):
+            table = self._table.data_ptr()
+        return self._lib.run_adamw_fn(self._handle, grads, table, s, stream)
 
     def __call__(self, step: Union[int, torch.Tensor], *, grads: Optional[Sequence[torch.Tensor]] = None,
                  lr: Union[None, float, torch.Tensor] = None, grad_scale: float = 1.0,
                  norm: Optional[torch.Tensor] = None, max_norm: Optional[float] = None, skip_nonfinite: bool = False,
                  seed: Optional[int] = None) -> None:
-        s = self._step(step, self._lr if lr is None else lr)
+        s = Step.from_buffer_copy(self._base)
+        if isinstance(step, torch.Tensor):
+            s.step_dev = _scalar(self._what, "step", step, torch.int64, self._device)
+        else:
+            s.step = step
+        if lr is not None:
+            self._set_lr(s, lr)
         s.grad_scale = grad_scale
         if norm is not None:
             s.norm = _scalar(self._what, "norm", norm, torch.float32, self._device)
@@ -183,51 +203,30 @@ class AdamWPlan(_Plan):
             if not max_norm > 0:
                 raise ValueError(f"{self._what}: max_norm must be positive, got {max_norm}")
             s.max_norm = max_norm
-        s.skip_nonfinite = 1 if skip_nonfinite else 0
+        if skip_nonfinite:
+            s.skip_nonfinite = 1
         if seed is not None:
             if not 0 <= seed < 1 << 32:
                 raise ValueError(f"{self._what}: seed must be in [0, 2**32), got {seed}")
             s.stochastic, s.seed = 1, seed
-        table = None
-        if grads is not None:
-            grads = list(grads)
-            if len(grads) != len(self._like):
-                raise ValueError(f"{self._what}: the plan has {len(self._like)} gradients, got {len(grads)}")
-            for i, (g, (n, shape, dtype)) in enumerate(zip(grads, self._like)):
-                kernels.check_device_tensor(g, f"grads[{i}]")
-                if g.dtype != dtype or g.numel() != n or (g.shape != shape and g.dim() > 1 and len(shape) > 1):
-                    raise RuntimeError(f"{self._what}: grads[{i}] must have the type and shape of the plan's "
-                                       f"({dtype}, {tuple(shape)}), got {g.dtype}, {tuple(g.shape)}")
-                _check_device(self._what, f"grads[{i}]", g, self._device)
-            table = _optim_native._ptr_table([g.data_ptr() for g in grads])
-        self._done(_on(self._device, self._run, table, s))
+        self._run(self._step, None if grads is None else self._other(grads), s)
 
-    def _run(self, grads, step, stream):
-        table = None
-        if self._table is not None and grads is None and stream == self._table_stream and not _capturing(self._device):
-            table = self._table.data_ptr()
-        return self._lib.run_adamw_fn(self._native.handle, grads, table, step, stream)
-
-    def _make_table(self):
-        """The addresses of more tensors than one launch takes in its arguments, in
-        device memory.  It is written, read and freed on ONE stream, the one the
-        plan is made on; calls on other streams and captured calls (a graph may
-        outlive the plan) pass the addresses in arguments, in a few launches."""
-        self._table = None
-        size = self._lib.table_bytes(self._native)
-        if not size or _capturing(self._device):
-            return
-        host = torch.empty(size, dtype=torch.uint8)
-        self._lib.table_fill(self._native, host.data_ptr(), size)
-
-        def put(stream):
-            self._table, self._table_stream = host.to(self._device), stream
-        _on(self._device, put)
+    def _other(self, grads):
+        grads = list(grads)
+        if len(grads) != len(self._like):
+            raise ValueError(f"{self._what}: the plan has {len(self._like)} gradients, got {len(grads)}")
+        for i, (g, (n, shape, dtype)) in enumerate(zip(grads, self._like)):
+            kernels.check_device_tensor(g, f"grads[{i}]")
+            if g.dtype != dtype or g.numel() != n or (g.shape != shape and g.dim() > 1 and len(shape) > 1):
+                raise RuntimeError(f"{self._what}: grads[{i}] must have the type and shape of the plan's "
+                                   f"({dtype}, {tuple(shape)}), got {g.dtype}, {tuple(g.shape)}")
+            _check_device(self._what, f"grads[{i}]", g, self._device)
+        return _optim_native._ptr_table([g.data_ptr() for g in grads])
 
 
 def _plan_adamw(what, eight, params, grads, first, second, scales, copies, lr, betas, eps, weight_decay):
     params = _check_list(what, "params", params)
-    device = _one_device(what, params)
+    device = params[0].device if params else None
     grads = _check_list(what, "grads", grads, params)
     names = ("exp_avg", "exp_avg_rms" if eight else "exp_avg_sq")
     dtype = CODE_DTYPE if eight else torch.float32
@@ -257,9 +256,7 @@ def _plan_adamw(what, eight, params, grads, first, second, scales, copies, lr, b
         native = lib.plan_adamw(ptrs(params), ptrs(grads), ptrs(first), ptrs(second), cptrs, n, ptypes, gtypes, ctypes_)
     written = params + [c for c in copies or () if c is not None]
     plan = AdamWPlan(lib, native, device, _hold(params, grads, first, second, copies, *(scales or ())), written)
-    plan._what = what
-    plan._prepare(eight, grads, lr, betas, eps, weight_decay)
-    plan._make_table()
+    plan._prepare(what, grads, lr, betas, eps, weight_decay)
     return plan
 
 
@@ -346,8 +343,7 @@ class GradNormPlan(_Plan):
         # graphs do not share them
         size = self._work
         work = torch.empty(size // 8, dtype=torch.float64, device=self._device) if size else None
-        self._done(_on(self._device, self._lib.run_norm_fn, self._native.handle, out.data_ptr(),
-                       None if work is None else work.data_ptr(), size))
+        self._run(self._lib.run_norm_fn, self._handle, out.data_ptr(), None if work is None else work.data_ptr(), size)
         return out
 
 
@@ -360,7 +356,7 @@ def plan_grad_norm(tensors: Sequence[torch.Tensor]) -> GradNormPlan:
     tensors = _check_list("grad_norm", "tensors", tensors)
     if not tensors:
         raise ValueError("grad_norm: need at least one tensor (it names the GPU)")
-    device = _one_device("grad_norm", tensors)
+    device = tensors[0].device
     lib = _optim_native.load()
     native = lib.plan_norm(kernels._ptrs(tensors), [t.numel() for t in tensors], _type_codes("grad_norm", "tensors", tensors))
     plan = GradNormPlan(lib, native, device, _hold(tensors))
@@ -381,13 +377,13 @@ class BlocksPlan(_Plan):
     """A conversion of fixed tensors; made by plan_quantize_blocks and plan_dequantize_blocks."""
 
     def __call__(self) -> None:
-        self._done(_on(self._device, self._lib.run_blocks_fn, self._native.handle))
+        self._run(self._lib.run_blocks_fn, self._handle)
 
 
 def _plan_blocks(what, codes, scales, tensors, root):
     quantize = what == "quantize_blocks"
     tensors = _check_list(what, "tensors", tensors)
-    device = _one_device(what, tensors)
+    device = tensors[0].device if tensors else None
     codes = _check_list(what, "codes", codes, tensors, CODE_DTYPE)
     scales = _check_scales(what, "scales", scales, tensors)
     types = _type_codes(what, "tensors", tensors)
