@@ -625,7 +625,7 @@ int pccl_optim_run_norm(const pccl_optim_plan* plan, float* out, void* work, siz
   double* part = (double*)work;
   for (const Batch& b : plan->batches) {
     with_type(b.p, NormLaunch{*plan, b, part, out, (hipStream_t)stream});
-    part += norm_grid(b.items);
+    if (need) part += norm_grid(b.items);
   }
   if (!norm_alone(*plan))
     PCCL_LAUNCH(k_norm_join, dim3(1), dim3(kWave), 0, (hipStream_t)stream, (const double*)work, norm_parts(*plan), out);

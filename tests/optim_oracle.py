@@ -100,8 +100,12 @@ def _mix(x):
 
 def noise(seed, step, n):
     """The 32 random bits of each of n elements."""
-    key = _mix(_mix(seed) + step)
-    mask, i = np.uint64(0xffffffff), np.arange(n, dtype=np.uint64)
+    return noise_at(seed, step, np.arange(n, dtype=np.uint64))
+
+
+def noise_at(seed, step, i):
+    """... of the elements with these indices (uint64)."""
+    key, mask = _mix(_mix(seed) + step), np.uint64(0xffffffff)
     x = ((i & mask) + np.uint64(key) + (i >> np.uint64(32)) * np.uint64(0x9e3779b1)) & mask
     x ^= x >> np.uint64(16)
     x = (x * np.uint64(0x7feb352d)) & mask

@@ -510,6 +510,16 @@ def test_norm(where, sizes, dtype, gap):
     assert torch.equal(got, again) and got.shape == (1,) and got.dtype == torch.float32
 
 
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+def test_norm_of_more_than_every_wave_takes_at_once(where, dtype):
+    from pccl import optim
+    gen = torch.Generator().manual_seed(35)
+    ts = [torch.randn(n, generator=gen).to(TYPES[dtype]).to(where.device) for n in (9000001, 13, 9500000)]
+    got = optim.grad_norm(ts)
+    where.sync()
+    check_norm(got, ts, "large")
+
+
 def test_norm_of_mixed_types(where):
     from pccl import optim
     gen = torch.Generator().manual_seed(32)
@@ -570,7 +580,7 @@ def block_buffers(sizes, device, gap):
 @pytest.mark.parametrize("gap", [0, 1, 3])
 @pytest.mark.parametrize("root", [False, True])
 @pytest.mark.parametrize("dtype", ["f32", "bf16", "f16"])
-@pytest.mark.parametrize("sizes", [EDGES, [256] * 130, [70001]])
+@pytest.mark.parametrize("sizes", [EDGES, [256] * 130, [70001], [3, 1700003, 500]])     # the last: several runs per die
 def test_blocks_there_and_back(where, sizes, dtype, root, gap):
     from pccl import optim
     gen = torch.Generator().manual_seed(41)
@@ -720,6 +730,50 @@ def test_a_sharded_step_over_virtual_ranks(where, monkeypatch):
             close(master[r], *res["p"], f"rank {r} step {step}")
             close(copy[r], res["p"][0], Q.rounded(*res["p"], torch.bfloat16), f"copy {r} step {step}")
             assert torch.equal(full[r], torch.cat(copy))
+
+
+def test_a_sharded_step_as_a_rank_program(where, monkeypatch):
+    """The same as every rank of a data-parallel program would write it: the norm of
+    all shards is the norm of the ranks' norms, gathered."""
+    import pccl
+    from pccl import _native, optim
+    if where.device == "cpu":
+        import conftest
+        monkeypatch.setattr(_native, "_loaded", _native.NativeLib(conftest.build_cpu_library()))
+    P, B, device = 4, 260, where.device
+    gen = torch.Generator().manual_seed(55)
+    grads = [torch.randn(P * B, generator=gen).to(torch.bfloat16).to(device) for _ in range(P)]
+    start = torch.randn(P * B, generator=gen).to(device)
+    full = [torch.zeros(P * B, dtype=torch.bfloat16, device=device) for _ in range(P)]
+    norms = [torch.zeros(P, device=device) for _ in range(P)]
+    kept = [None] * P
+
+    def rank_main(comm):
+        r = comm.Get_rank()
+        shard = torch.empty(B, dtype=torch.bfloat16, device=device)
+        pccl.reduce_scatter_mpi(shard, grads[r], comm, "ring")
+        mine = optim.grad_norm([shard])
+        pccl.all_gather_mpi(norms[r], mine, comm, "ring")
+        norm = optim.grad_norm([norms[r]])
+        master = start[r * B:(r + 1) * B].clone()
+        m, ms = optim.empty_blocks(master)
+        v, vs = optim.empty_blocks(master)
+        copy = torch.empty(B, dtype=torch.bfloat16, device=device)
+        optim.adamw8([master], [shard], [m], [v], [ms], [vs], 1, seed=r, copies=[copy], grad_scale=1 / P, norm=norm, max_norm=1.0,
+                     **HYPER)
+        pccl.all_gather_mpi(full[r], copy, comm, "ring")
+        kept[r] = (shard, norm, copy)
+    pccl.VirtualWorld(P, device).run(rank_main)
+    where.sync()
+    shards = [k[0] for k in kept]
+    whole = np.concatenate([f64(t) for t in shards])
+    for r in range(P):
+        assert abs(float(kept[r][1]) - np.linalg.norm(whole)) <= 8 * U * np.linalg.norm(whole)
+        zero = np.zeros(B)
+        res = Q.adamw(f64(start[r * B:(r + 1) * B]), f64(shards[r]), zero, zero, 1, norm=float(kept[r][1]), max_norm=1.0,
+                      grad_scale=1 / P, **HYPER)
+        close(kept[r][2], res["p"][0], Q.rounded(*res["p"], torch.bfloat16), f"rank {r}")
+        assert torch.equal(full[r], torch.cat([k[2] for k in kept]))
 
 
 def test_the_norm_of_norms_is_the_norm(where):
@@ -1104,6 +1158,76 @@ def test_one_plan_from_several_threads():
         t.join()
     assert not errors, errors
     del s, gs
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("eight", [False, True])
+def test_a_plan_of_many_tensors_on_other_streams_and_in_a_graph_that_outlives_it(eight):
+    """The table in device memory is used on the plan's own stream alone; elsewhere the results are the same."""
+    from pccl import optim
+    dev, sizes = "cuda:0", [300 + k for k in range(150)]
+    keys = ("p", "g", "m", "r", "ms", "rs") if eight else ("p", "g", "m", "v")
+    def fresh():
+        s = make(sizes, dev, seed=64, eight=eight)
+        return s, (optim.plan_adamw8 if eight else optim.plan_adamw)(*(s[k].list for k in keys), **HYPER)
+    a, plan_a = fresh()
+    b, plan_b = fresh()
+    assert plan_a._table is not None
+    side = torch.cuda.Stream()
+    torch.cuda.synchronize()
+    plan_a(1)
+    with torch.cuda.stream(side):
+        plan_b(1)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        plan_b(2)
+    del plan_b
+    for _ in range(3):
+        junk = [torch.full((1 << 20,), 255, dtype=torch.uint8, device=dev) for _ in range(8)]     # where the plan's table was
+        plan_a(2)
+        graph.replay()
+        torch.cuda.synchronize()
+        del junk
+    for k in keys:
+        assert np.array_equal(Flat.raw(a[k].flat), Flat.raw(b[k].flat)), k
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("eight", [False, True])
+def test_adamw_offsets_beyond_32_bits(eight):
+    """A tensor of more than 2^32 elements, zero but for a few: they are stepped, and nothing else is."""
+    from pccl import optim
+    dev, n = "cuda:0", (1 << 32) + 1000
+    if torch.cuda.mem_get_info()[0] < 120 << 30:
+        pytest.skip("needs 120 GiB of free GPU memory")
+    at = torch.tensor([0, 5, (1 << 31) + 7, (1 << 32) - 1, 1 << 32, n - 2, n - 1], device=dev)
+    p, g = torch.zeros(n, dtype=torch.bfloat16, device=dev), torch.zeros(n, dtype=torch.bfloat16, device=dev)
+    p[at], g[at] = 0.5, torch.tensor([1.0, 0.25, -2.0, 3.0, 0.75, -0.3, 1.0], device=dev).to(torch.bfloat16)
+    old = f64(p[at]), f64(g[at])
+    if eight:
+        m, ms = optim.empty_blocks(p)
+        v, vs = optim.empty_blocks(p)
+        optim.adamw8([p], [g], [m], [v], [ms], [vs], 1, seed=9, **HYPER)
+    else:
+        m, v = (torch.zeros(n, device=dev) for _ in range(2))
+        optim.adamw([p], [g], [m], [v], 1, **HYPER)
+    torch.cuda.synchronize()
+    zero = np.zeros(at.numel())
+    r = Q.adamw(*old, zero, zero, 1, **HYPER)
+    close(p[at], r["p"][0], Q.rounded(*r["p"], torch.bfloat16), "parameters")
+    assert int((p != 0).sum()) == at.numel()
+    if not eight:
+        close(m[at], *r["m"], "first moments")
+        assert int((m != 0).sum()) == at.numel() and int((v != 0).sum()) == at.numel()
+        return
+    # of the last two elements of the tensor the smaller one is rounded by the random bits of its own index
+    i = np.array([n - 2, n - 1], dtype=np.uint64)
+    bits = Q.noise_at(9, 1, i)
+    y = np.abs(r["m"][0][5:]) / (np.abs(r["m"][0][5:]).max() / 448)
+    want = np.floor(y / Q.spacing(y) + (bits & np.uint64(0xffff)).astype(float) / 65536) * Q.spacing(y)
+    assert np.abs(f64(m[at[5:]].float())).tolist() == want.tolist()
+    assert int((m.view(torch.uint8) & 0x7f != 0).sum()) == at.numel() and int((v.view(torch.uint8) != 0).sum()) == at.numel()
 
 
 @pytest.mark.gpu
