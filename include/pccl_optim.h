@@ -40,8 +40,9 @@ extern "C" {
 /* Elements that share one scale in the 8-bit form. */
 #define PCCL_OPTIM_BLOCK 256
 
-/* Longest tensor: 2^26 - 1 workgroups of one launch, 256 elements each. */
-#define PCCL_OPTIM_MAX_ELEMENTS (((size_t)1 << 34) - 256)
+/* Longest tensor: 2^26 - 1 workgroups of one launch, 256 elements each, the
+ * first and the last of them possibly not whole. */
+#define PCCL_OPTIM_MAX_ELEMENTS (((size_t)1 << 34) - 512)
 
 /* In place of an element type: no copy for this tensor. */
 #define PCCL_OPTIM_NONE (-1)
@@ -117,12 +118,17 @@ int pccl_optim_run_adamw(const pccl_optim_plan* plan, const void* const* grads, 
  * out[0] = sqrt(sum of x^2 over all elements of all tensors), fp32; 0 for no
  * elements.  Squares of huge and of tiny values neither overflow nor vanish;
  * the partial sums are kept in 64 bits and joined in a fixed order, so equal
- * inputs give equal bits.  Inf or NaN anywhere gives inf or NaN.  `work`:
- * pccl_optim_norm_work(plan) bytes (may be 0) of device memory, 8-byte aligned,
- * that nothing else uses until the launch is done; its contents do not matter. */
+ * inputs give equal bits.  Inf or NaN anywhere gives inf or NaN.
+ * `work`: pccl_optim_norm_work(plan) bytes (may be 0) of device memory, 8-byte
+ * aligned, that nothing else uses until the launch is done; its contents do not
+ * matter.  `ticket`: NULL, or PCCL_OPTIM_TICKET_BYTES of device memory that are
+ * all 0 and are 0 again afterwards; the norm then takes one launch where it
+ * takes two without, with the same result.  Runs that share a ticket must not
+ * overlap.  Neither out, work nor ticket may lie in the tensors. */
+#define PCCL_OPTIM_TICKET_BYTES 576
 int pccl_optim_plan_norm(pccl_optim_plan** plan, const void* const* tensors, const size_t* n, const int* dtype, int count);
 size_t pccl_optim_norm_work(const pccl_optim_plan* plan);
-int pccl_optim_run_norm(const pccl_optim_plan* plan, float* out, void* work, size_t work_bytes, void* stream);
+int pccl_optim_run_norm(const pccl_optim_plan* plan, float* out, void* work, size_t work_bytes, uint32_t* ticket, void* stream);
 
 /* ---- 8-bit blocks --------------------------------------------------------
  * Blocks of 256 consecutive elements from the start of each tensor, the last

@@ -105,7 +105,8 @@ struct pccl_optim_plan {
   std::vector<size_t> n;
   std::vector<int> gtype;
   std::vector<Batch> batches;
-  std::vector<Extent> written;           // what the plan writes, by address
+  std::vector<Extent> guarded;           // what a buffer that a run brings must not lie in, by address: what the plan
+                                         // writes, and what a norm reads
 };
 
 namespace {
@@ -145,20 +146,23 @@ struct Checker {
       if (x.written && far && far->hi > x.lo) return clash(what, *far, x);
       if (far_written && far_written->hi > x.lo) return clash(what, *far_written, x);
       if (!far || x.hi > far->hi) far = &x;
-      if (x.written) { far_written = &x; plan.written.push_back(x); }
+      if (x.written) far_written = &x;
+      if (plan.kind == kNorm && !plan.guarded.empty() && plan.guarded.back().hi >= x.lo)
+        plan.guarded.back().hi = std::max(plan.guarded.back().hi, x.hi);   // readers may overlap; kept apart and in order
+      else if (x.written || plan.kind == kNorm) plan.guarded.push_back(x);
     }
     return PCCL_HIP_OK;
   }
 };
 
-// A buffer that a run brings along must not lie in what the plan writes.
+// A buffer that a run brings along must not lie in what the plan guards.
 int check_apart(const pccl_optim_plan& plan, const void* p, size_t bytes, const char* name, int i, const char* what) {
   if (!p || !bytes) return PCCL_HIP_OK;
   const Extent x{(uintptr_t)p, (uintptr_t)p + bytes, i, name, false};
-  auto it = std::upper_bound(plan.written.begin(), plan.written.end(), x,
+  auto it = std::upper_bound(plan.guarded.begin(), plan.guarded.end(), x,
                              [](const Extent& u, const Extent& v) { return u.lo < v.lo; });
-  if (it != plan.written.end() && it->lo < x.hi) return Checker::clash(what, *it, x);
-  if (it != plan.written.begin() && (--it)->hi > x.lo) return Checker::clash(what, *it, x);
+  if (it != plan.guarded.end() && it->lo < x.hi) return Checker::clash(what, *it, x);
+  if (it != plan.guarded.begin() && (--it)->hi > x.lo) return Checker::clash(what, *it, x);
   return PCCL_HIP_OK;
 }
 
@@ -476,18 +480,22 @@ uint32_t norm_parts(const pccl_optim_plan& plan) {
 struct NormLaunch {
   const pccl_optim_plan& plan;
   const Batch& b;
-  double* part;
+  double* all;
+  uint32_t done;        // partial sums of the launches before this one
+  uint32_t* ticket;     // of the last launch only
   float* out;
   hipStream_t stream;
   template <class T> void operator()() const {
+    const uint32_t parts = norm_parts(plan);
     // a batch of a norm is never longer than a table in kernel arguments
     each_launch<NormTable>(plan, b, nullptr, nullptr, [&](const NormTable& t, const Share& s) {
+      const dim3 grid(norm_alone(plan) ? 1 : norm_grid(s.items)), block(kNormThreads);
       if (norm_alone(plan))
-        PCCL_LAUNCH((k_sum_squares<T, kNormThreads, false, true>), dim3(1), dim3(kNormThreads), 0, stream, t, s.count, s.items, part, out);
+        PCCL_LAUNCH((k_sum_squares<T, kNormThreads, false, true>), grid, block, 0, stream, t, s.count, s.items, all, parts, done, ticket, out);
       else if (plan.stream)
-        PCCL_LAUNCH((k_sum_squares<T, kNormThreads, true, false>), dim3(norm_grid(s.items)), dim3(kNormThreads), 0, stream, t, s.count, s.items, part, out);
+        PCCL_LAUNCH((k_sum_squares<T, kNormThreads, true, false>), grid, block, 0, stream, t, s.count, s.items, all, parts, done, ticket, out);
       else
-        PCCL_LAUNCH((k_sum_squares<T, kNormThreads, false, false>), dim3(norm_grid(s.items)), dim3(kNormThreads), 0, stream, t, s.count, s.items, part, out);
+        PCCL_LAUNCH((k_sum_squares<T, kNormThreads, false, false>), grid, block, 0, stream, t, s.count, s.items, all, parts, done, ticket, out);
     });
   }
 };
@@ -613,21 +621,26 @@ size_t pccl_optim_norm_work(const pccl_optim_plan* plan) {
   return plan && plan->kind == kNorm ? (size_t)norm_parts(*plan) * sizeof(double) : 0;
 }
 
-int pccl_optim_run_norm(const pccl_optim_plan* plan, float* out, void* work, size_t work_bytes, void* stream) {
+int pccl_optim_run_norm(const pccl_optim_plan* plan, float* out, void* work, size_t work_bytes, uint32_t* ticket, void* stream) {
   const char* what = "pccl_optim_run_norm";
   if (int rc = check_plan(plan, what, kNorm, kNorm)) return rc;
   if (!out) return fail(PCCL_HIP_EINVAL, "%s: out is NULL", what);
   if ((uintptr_t)out % 4) return fail(PCCL_HIP_EINVAL, "%s: out is not aligned to 4 bytes", what);
+  if ((uintptr_t)ticket % 4) return fail(PCCL_HIP_EINVAL, "%s: ticket is not aligned to 4 bytes", what);
   const size_t need = pccl_optim_norm_work(plan);
   if (need && (!work || work_bytes < need))
     return fail(PCCL_HIP_EINVAL, "%s: needs %zu bytes of work space, got %zu", what, need, work ? work_bytes : (size_t)0);
   if (need && (uintptr_t)work % sizeof(double)) return fail(PCCL_HIP_EINVAL, "%s: work is not aligned to 8 bytes", what);
-  double* part = (double*)work;
+  const struct { const void* p; size_t bytes; const char* name; } own[] = {{out, 4, "out"}, {need ? work : nullptr, need, "work"}, {ticket, PCCL_OPTIM_TICKET_BYTES, "ticket"}};
+  for (const auto& x : own)
+    if (int rc = check_apart(*plan, x.p, x.bytes, x.name, 0, what)) return rc;
+  uint32_t done = 0;
   for (const Batch& b : plan->batches) {
-    with_type(b.p, NormLaunch{*plan, b, part, out, (hipStream_t)stream});
-    if (need) part += norm_grid(b.items);
+    const bool last = &b == &plan->batches.back();
+    with_type(b.p, NormLaunch{*plan, b, (double*)work, done, last ? ticket : nullptr, out, (hipStream_t)stream});
+    done += norm_grid(b.items);
   }
-  if (!norm_alone(*plan))
+  if (plan->batches.empty() || (!ticket && !norm_alone(*plan)))
     PCCL_LAUNCH(k_norm_join, dim3(1), dim3(kWave), 0, (hipStream_t)stream, (const double*)work, norm_parts(*plan), out);
   return launch_status(what);
 }

@@ -804,7 +804,6 @@ __device__ __forceinline__ double group_sum(const double* part) {
   __shared__ double waves[T / kWave];
   double x = part[0];
   for (int d = kWave / 2; d; d >>= 1) x += __shfl_xor(x, d);
-  if constexpr (T == kWave) return x;
   if ((threadIdx.x & (kWave - 1)) == 0) waves[threadIdx.x / kWave] = x;
   __syncthreads();
   double sum = 0;
@@ -844,11 +843,83 @@ template <int N, class V> __device__ __forceinline__ double sum_squares(const V&
   return sum;
 }
 
-// One partial sum per workgroup of T threads; every wave walks the work items
-// that lie as many apart as the grid has waves.
-// FINAL: the only workgroup of the whole norm; it writes the result itself.
-template <class E, int T, bool NT, bool FINAL>
-__global__ __launch_bounds__(T) void k_sum_squares(NormTable args, int count, uint32_t items, double* part, float* out) {
+// The partial sums, added up by the first wave of a workgroup in a fixed order;
+// valid in thread 0.  They may have been written by other workgroups of the same
+// launch on other dies, so they are read past the caches.
+__device__ __forceinline__ double join_parts(const double* part, uint32_t count) {
+  double sum[kLaneSlots];
+  each_lane([&](int k, int lane) {
+    double acc = 0;
+#pragma unroll 4
+    for (uint32_t i = lane; i < count; i += kWave) {
+#if defined(__HIP_DEVICE_COMPILE__)
+      acc += __hip_atomic_load(part + i, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+#else
+      acc += part[i];
+#endif
+    }
+    sum[k] = acc;
+  });
+#if defined(__HIP_DEVICE_COMPILE__)
+  for (int d = kWave / 2; d; d >>= 1) sum[0] += __shfl_xor(sum[0], d);
+  return sum[0];
+#else
+  double total = 0;
+  for (int l = 0; l < kWave; ++l) total += sum[l];
+  return total;
+#endif
+}
+
+// Writes a workgroup's partial sum and says to all its threads whether it was
+// the last of the launch to do so.  The workgroups of a die count themselves at
+// one place each, and the last ones of the dies at another: additions to one
+// address take about 10 ns each, and 256 of them in a row were 2.5 us.  The
+// counters, 64 bytes apart, are 0 before the launch and again after it.
+constexpr uint32_t kTicketStep = 16;
+static_assert(PCCL_OPTIM_TICKET_BYTES == (1 + kXcds) * kTicketStep * 4, "a counter per die, and one for the dies");
+
+__device__ __forceinline__ bool last_to_write(double* part, double sum, uint32_t* ticket) {
+  const uint32_t die = blockIdx.x % kXcds;
+  const uint32_t of_die = (gridDim.x - die + kXcds - 1) / kXcds, dies = gridDim.x < kXcds ? gridDim.x : kXcds;
+  uint32_t* const mine = ticket + (1 + die) * kTicketStep;
+#if defined(__HIP_DEVICE_COMPILE__)
+  __shared__ bool last;
+  if (threadIdx.x == 0) {
+    // All accesses are made where the dies meet, and the store is done when the counters say so.  (A release would
+    // write the die's whole L2 back for it: 6 us on a norm of 1 GiB.)
+    __hip_atomic_store(part, sum, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    last = false;
+    if (__hip_atomic_fetch_add(mine, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == of_die - 1) {
+      __hip_atomic_store(mine, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+      if (__hip_atomic_fetch_add(ticket, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == dies - 1) {
+        __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "agent");
+        __hip_atomic_store(ticket, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        last = true;
+      }
+    }
+  }
+  __syncthreads();
+  return last;
+#else
+  *part = sum;
+  if (++*mine < of_die) return false;
+  *mine = 0;
+  if (++*ticket < dies) return false;
+  *ticket = 0;
+  return true;
+#endif
+}
+
+// One partial sum per workgroup of T threads, to all[done + blockIdx.x]; every wave
+// walks the work items that lie as many apart as the grid has waves.
+// ALONE: the only workgroup of the whole norm; it writes the result itself.
+// With a ticket the last workgroup to finish adds up the `parts` partial sums of
+// this and the launches before it and writes the result;
+// without one k_norm_join does, with the same bits, in a launch more.
+template <class E, int T, bool NT, bool ALONE>
+__global__ __launch_bounds__(T) void k_sum_squares(NormTable args, int count, uint32_t items, double* all, uint32_t parts,
+                                                   uint32_t done, uint32_t* ticket, float* out) {
   if (kHostRun && threadIdx.x) return;
   typedef Vec16<E> V;
   typedef typename E::elem elem;
@@ -892,24 +963,20 @@ __global__ __launch_bounds__(T) void k_sum_squares(NormTable args, int count, ui
     sum[k] = acc;
   }
   const double total = group_sum<T>(sum);
-  if (threadIdx.x == 0) {
-    if constexpr (FINAL) out[0] = (float)sqrt(total);
-    else part[blockIdx.x] = total;
+  if constexpr (ALONE) {
+    if (threadIdx.x == 0) out[0] = (float)sqrt(total);
+  } else if (!ticket) {
+    if (threadIdx.x == 0) all[done + blockIdx.x] = total;
+  } else if (last_to_write(all + done + blockIdx.x, total, ticket) && threadIdx.x < kWave) {
+    const double norm2 = join_parts(all, parts);
+    if (threadIdx.x == 0) out[0] = (float)sqrt(norm2);
   }
 }
 
-// One wave adds the partial sums up.
-__global__ __launch_bounds__(kWave) void k_norm_join(const double* part, uint32_t count, float* out) {
+__global__ __launch_bounds__(kWave) void k_norm_join(const double* all, uint32_t parts, float* out) {
   if (kHostRun && threadIdx.x) return;
-  double sum[kLaneSlots];
-  each_lane([&](int k, int lane) {
-    double acc = 0;
-#pragma unroll 4
-    for (uint32_t i = lane; i < count; i += kWave) acc += part[i];
-    sum[k] = acc;
-  });
-  const double total = group_sum<kWave>(sum);
-  if (threadIdx.x == 0) out[0] = (float)sqrt(total);
+  const double norm2 = join_parts(all, parts);
+  if (threadIdx.x == 0) out[0] = (float)sqrt(norm2);
 }
 
 }  // namespace pccl_optim_kernels

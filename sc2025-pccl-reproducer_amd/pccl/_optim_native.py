@@ -12,7 +12,8 @@ from typing import Optional, Sequence
 from ._native import LIB_PATH, NativeError, _ptr_table, _size_table
 
 BLOCK = 256                       # elements that share one scale
-MAX_ELEMENTS = (1 << 34) - 256    # of one tensor
+MAX_ELEMENTS = (1 << 34) - 512    # of one tensor
+TICKET_BYTES = 576                # counters of a norm in one launch
 NONE = -1                         # in place of an element type: no copy
 
 _vp = ctypes.c_void_p
@@ -42,7 +43,7 @@ SIGNATURES = {
     "pccl_optim_run_adamw": (_int, [_vp, _vpp, _vp, ctypes.POINTER(Step), _vp]),
     "pccl_optim_plan_norm": (_int, [_vpp, _vpp, _szp, _intp, _int]),
     "pccl_optim_norm_work": (_sz, [_vp]),
-    "pccl_optim_run_norm": (_int, [_vp, _vp, _vp, _sz, _vp]),
+    "pccl_optim_run_norm": (_int, [_vp, _vp, _vp, _sz, _vp, _vp]),
     "pccl_optim_plan_quantize": (_int, [_vpp, _vpp, _vpp, _vpp, _szp, _intp, _int, _int]),
     "pccl_optim_plan_dequantize": (_int, [_vpp, _vpp, _vpp, _vpp, _szp, _intp, _int, _int]),
     "pccl_optim_run_blocks": (_int, [_vp, _vp]),
@@ -132,8 +133,8 @@ class OptimLib:
     def norm_work(self, plan: Plan) -> int:
         return self._lib.pccl_optim_norm_work(plan.handle)
 
-    def run_norm(self, plan: Plan, out, work=0, work_bytes=0, stream=0):
-        self.check(self.run_norm_fn(plan.handle, out, work, work_bytes, stream))
+    def run_norm(self, plan: Plan, out, work=0, work_bytes=0, ticket=0, stream=0):
+        self.check(self.run_norm_fn(plan.handle, out, work, work_bytes, ticket, stream))
 
     def run_blocks(self, plan: Plan, stream=0):
         self.check(self.run_blocks_fn(plan.handle, stream))

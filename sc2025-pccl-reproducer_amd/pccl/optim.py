@@ -17,9 +17,10 @@ parameter new storage (`.data = ...`) and it needs a new plan.
 
 Like the rest of the package every call validates on the host, enqueues on the
 current stream of the tensors' device and returns; nothing synchronises, nothing
-runs on the CPU.  Calls may be captured into a graph: plans hold no device
-memory, and the step count and learning rate can live in device tensors so that
-a replay reads them anew.
+runs on the CPU.  Tensors are contiguous; they may start anywhere.  Calls may be
+captured into a graph, which may outlive the plan but not the tensors; the step
+count and learning rate can live in device tensors so that a replay reads them
+anew.
 """
 from __future__ import annotations
 
@@ -28,7 +29,7 @@ from typing import Optional, Sequence, Tuple, Union
 import torch
 
 from . import _optim_native, kernels
-from ._optim_native import BLOCK, Step
+from ._optim_native import BLOCK, TICKET_BYTES, Step
 
 CODE_DTYPE = torch.float8_e4m3fn      # of the 8-bit codes
 
@@ -141,6 +142,20 @@ class _Plan:
         if self._written:
             _increment_version(self._written)
 
+    # Some plans keep device memory of their own.  It is written, read and freed on
+    # ONE stream, the one the plan was made on; calls on other streams and captured
+    # calls (a graph may outlive the plan) do without it.
+    _own = _own_stream = None
+
+    def _make_own(self, make):
+        if not _capturing(self._index):
+            def put(stream):
+                self._own, self._own_stream = make(), stream
+            self._on_device(put)
+
+    def _usable(self, stream):
+        return self._own is not None and stream == self._own_stream and not _capturing(self._index)
+
 
 # ---------------------------------------------------------------------------
 # AdamW
@@ -149,13 +164,14 @@ class _Plan:
 class AdamWPlan(_Plan):
     """One AdamW step over fixed tensors; made by plan_adamw and plan_adamw8."""
 
-    def _prepare(self, what, grads, lr, betas, eps, weight_decay):
+    def _prepare(self, what, grads, lr, betas, eps, weight_decay, table):
         self._what = what
         self._like = [(g.numel(), g.shape, g.dtype) for g in grads]      # for calls that bring other gradients
         self._base = Step(beta1=betas[0], beta2=betas[1], eps=eps, weight_decay=weight_decay, grad_scale=1.0)
         self._set_lr(self._base, lr)
         self._keep.append(lr)
-        self._make_table()
+        if table:
+            self._make_table()
 
     def _set_lr(self, s, lr):
         if isinstance(lr, torch.Tensor):
@@ -164,25 +180,17 @@ class AdamWPlan(_Plan):
             s.lr_dev, s.lr = None, lr
 
     def _make_table(self):
-        """The addresses of more tensors than one launch takes in its arguments, in
-        device memory.  It is written, read and freed on ONE stream, the one the
-        plan is made on; calls on other streams and captured calls (a graph may
-        outlive the plan) pass the addresses in arguments, in a few launches."""
-        self._table = self._table_stream = None
+        """The addresses of more tensors than one launch takes in its arguments, in device memory."""
         size = self._lib.table_bytes(self._native)
-        if not size or _capturing(self._index):
+        if not size:
             return
-        host = torch.empty(size, dtype=torch.uint8)
+        pinned = self._index is not None
+        host = torch.empty(size, dtype=torch.uint8, pin_memory=pinned)
         self._lib.table_fill(self._native, host.data_ptr(), size)
-
-        def put(stream):
-            self._table, self._table_stream = host.to(self._device), stream
-        self._on_device(put)
+        self._make_own(lambda: host.to(self._device, non_blocking=True) if pinned else host)
 
     def _step(self, grads, s, stream):
-        table = None
-        if self._table is not None and grads is None and stream == self._table_stream and not _capturing(self._index):
-            table = self._table.data_ptr()
+        table = self._own.data_ptr() if grads is None and self._usable(stream) else None
         return self._lib.run_adamw_fn(self._handle, grads, table, s, stream)
 
     def __call__(self, step: Union[int, torch.Tensor], *, grads: Optional[Sequence[torch.Tensor]] = None,
@@ -224,7 +232,7 @@ class AdamWPlan(_Plan):
         return _optim_native._ptr_table([g.data_ptr() for g in grads])
 
 
-def _plan_adamw(what, eight, params, grads, first, second, scales, copies, lr, betas, eps, weight_decay):
+def _plan_adamw(what, eight, params, grads, first, second, scales, copies, lr, betas, eps, weight_decay, table=True):
     params = _check_list(what, "params", params)
     device = params[0].device if params else None
     grads = _check_list(what, "grads", grads, params)
@@ -256,7 +264,7 @@ def _plan_adamw(what, eight, params, grads, first, second, scales, copies, lr, b
         native = lib.plan_adamw(ptrs(params), ptrs(grads), ptrs(first), ptrs(second), cptrs, n, ptypes, gtypes, ctypes_)
     written = params + [c for c in copies or () if c is not None]
     plan = AdamWPlan(lib, native, device, _hold(params, grads, first, second, copies, *(scales or ())), written)
-    plan._prepare(what, grads, lr, betas, eps, weight_decay)
+    plan._prepare(what, grads, lr, betas, eps, weight_decay, table)
     return plan
 
 
@@ -313,18 +321,18 @@ def plan_adamw8(params: Sequence[torch.Tensor], grads: Sequence[torch.Tensor], e
 def adamw(params, grads, exp_avg, exp_avg_sq, step, *, copies=None, lr=1e-3, betas=(0.9, 0.999), eps=1e-8,
           weight_decay=1e-2, grad_scale=1.0, norm=None, max_norm=None, skip_nonfinite=False) -> None:
     """One AdamW step; see plan_adamw."""
-    plan_adamw(params, grads, exp_avg, exp_avg_sq, copies=copies, lr=lr, betas=betas, eps=eps,
-               weight_decay=weight_decay)(step, grad_scale=grad_scale, norm=norm, max_norm=max_norm,
-                                          skip_nonfinite=skip_nonfinite)
+    plan = _plan_adamw("adamw", False, params, grads, exp_avg, exp_avg_sq, None, copies, lr, betas, eps, weight_decay,
+                       table=False)
+    plan(step, grad_scale=grad_scale, norm=norm, max_norm=max_norm, skip_nonfinite=skip_nonfinite)
 
 
 def adamw8(params, grads, exp_avg, exp_avg_rms, avg_scale, rms_scale, step, *, seed=None, copies=None, lr=1e-3,
            betas=(0.9, 0.999), eps=1e-8, weight_decay=1e-2, grad_scale=1.0, norm=None, max_norm=None,
            skip_nonfinite=False) -> None:
     """One AdamW step with moments in 8 bits; see plan_adamw8."""
-    plan_adamw8(params, grads, exp_avg, exp_avg_rms, avg_scale, rms_scale, copies=copies, lr=lr, betas=betas, eps=eps,
-                weight_decay=weight_decay)(step, grad_scale=grad_scale, norm=norm, max_norm=max_norm,
-                                           skip_nonfinite=skip_nonfinite, seed=seed)
+    plan = _plan_adamw("adamw8", True, params, grads, exp_avg, exp_avg_rms, (avg_scale, rms_scale), copies, lr, betas, eps,
+                       weight_decay, table=False)
+    plan(step, grad_scale=grad_scale, norm=norm, max_norm=max_norm, skip_nonfinite=skip_nonfinite, seed=seed)
 
 
 # ---------------------------------------------------------------------------
@@ -334,16 +342,27 @@ def adamw8(params, grads, exp_avg, exp_avg_rms, avg_scale, rms_scale, step, *, s
 class GradNormPlan(_Plan):
     """The norm of fixed tensors; made by plan_grad_norm."""
 
+    def _prepare(self, keep_work):
+        self._size = self._lib.norm_work(self._native)
+        if self._size and keep_work:       # the partial sums and, behind them, the ticket
+            self._make_own(lambda: torch.zeros(self._size + TICKET_BYTES, dtype=torch.uint8, device=self._device))
+
+    def _norm(self, out, stream):
+        if not self._size:
+            return self._lib.run_norm_fn(self._handle, out, None, 0, None, stream)
+        if self._usable(stream):
+            at = self._own.data_ptr()
+            return self._lib.run_norm_fn(self._handle, out, at, self._size, at + self._size, stream)
+        # partial sums of this call alone: two streams or two graphs do not share them
+        work = torch.empty(self._size // 8, dtype=torch.float64, device=self._device)
+        return self._lib.run_norm_fn(self._handle, out, work.data_ptr(), self._size, None, stream)
+
     def __call__(self, out: Optional[torch.Tensor] = None) -> torch.Tensor:
         if out is None:
             out = torch.empty(1, dtype=torch.float32, device=self._device)
         else:
             _scalar("grad_norm", "out", out, torch.float32, self._device)
-        # partial sums of this call alone: from the allocator, so that calls on two streams or captured into two
-        # graphs do not share them
-        size = self._work
-        work = torch.empty(size // 8, dtype=torch.float64, device=self._device) if size else None
-        self._run(self._lib.run_norm_fn, self._handle, out.data_ptr(), None if work is None else work.data_ptr(), size)
+        self._run(self._norm, out.data_ptr())
         return out
 
 
@@ -353,6 +372,10 @@ def plan_grad_norm(tensors: Sequence[torch.Tensor]) -> GradNormPlan:
     tensor on the GPU, or writes it into the one given.  No sum over- or
     underflows; inf or NaN among the elements gives inf or NaN; equal inputs give
     equal bits.  The norm over several ranks is the norm of their norms."""
+    return _plan_grad_norm(tensors, True)
+
+
+def _plan_grad_norm(tensors, keep_work):
     tensors = _check_list("grad_norm", "tensors", tensors)
     if not tensors:
         raise ValueError("grad_norm: need at least one tensor (it names the GPU)")
@@ -360,13 +383,13 @@ def plan_grad_norm(tensors: Sequence[torch.Tensor]) -> GradNormPlan:
     lib = _optim_native.load()
     native = lib.plan_norm(kernels._ptrs(tensors), [t.numel() for t in tensors], _type_codes("grad_norm", "tensors", tensors))
     plan = GradNormPlan(lib, native, device, _hold(tensors))
-    plan._work = lib.norm_work(native)
+    plan._prepare(keep_work)
     return plan
 
 
 def grad_norm(tensors: Sequence[torch.Tensor], out: Optional[torch.Tensor] = None) -> torch.Tensor:
     """The 2-norm over all elements of all tensors; see plan_grad_norm."""
-    return plan_grad_norm(tensors)(out)
+    return _plan_grad_norm(tensors, False)(out)
 
 
 # ---------------------------------------------------------------------------

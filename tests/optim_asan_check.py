@@ -102,6 +102,11 @@ for lengths in (LENGTHS, [7] * 150, [300]):
             plan = lib.plan_norm(x, lengths, [code] * count)
             out = np.zeros(1, np.float32)
             work = np.zeros(lib.norm_work(plan), np.uint8)
-            lib.run_norm(plan, out.ctypes.data, work.ctypes.data if work.size else 0, work.size)
-            checked += 1
+            ticket = np.zeros(nat.TICKET_BYTES, np.uint8)
+            both = []
+            for counter in (0, ticket.ctypes.data):
+                lib.run_norm(plan, out.ctypes.data, work.ctypes.data if work.size else 0, work.size, counter)
+                both.append(out.tobytes())
+            assert both[0] == both[1] and not ticket.any()
+            checked += 2
 print("ASAN CHECK OK", checked)

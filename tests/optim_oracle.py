@@ -26,9 +26,11 @@ def cpu_library(out=os.path.join(ROOT, "tests", "build", "libpccl_optim_cpu.so")
     if not os.path.exists(HOST_CLANG):
         pytest.skip("host clang++ of the ROCm toolchain not found")
     os.makedirs(os.path.dirname(out), exist_ok=True)
+    part = f"{out}.{os.getpid()}"          # put in place whole: test processes may build it side by side
     subprocess.run([HOST_CLANG, "-x", "c++", "-std=c++17", "-g", "-fPIC", "-shared", "-ffp-contract=off", *flags,
                     "-I", os.path.join(ROOT, "tests", "hip_cpu_shim"), "-I", os.path.join(ROOT, "include"), "-I", CSRC,
-                    "-o", out, srcs[0]], check=True, capture_output=True)
+                    "-o", part, srcs[0]], check=True, capture_output=True)
+    os.replace(part, out)
     return out
 
 

@@ -288,7 +288,7 @@ def test_many_tensors_of_one_type(where, count, eight):
     other = make(sizes, where.device, g="bf16", gap=2, seed=16)
     keys = ("p", "g", "m", "r", "ms", "rs") if eight else ("p", "g", "m", "v")
     plan = (optim.plan_adamw8 if eight else optim.plan_adamw)(*(s[k].list for k in keys), copies=s["c"].list, **HYPER)
-    assert (plan._table is not None) == (sum(n > 0 for n in sizes) > (56 if eight else 64))
+    assert (plan._own is not None) == (sum(n > 0 for n in sizes) > (56 if eight else 64))
     check, read = (check_adamw8, values8) if eight else (check_adamw, lambda s: values(s, "pgmv"))
     old = read(s)
     plan(3)
@@ -507,7 +507,9 @@ def test_norm(where, sizes, dtype, gap):
     assert plan(again) is again
     where.sync()
     check_norm(got, s.list, "norm")
-    assert torch.equal(got, again) and got.shape == (1,) and got.dtype == torch.float32
+    once = optim.grad_norm(s.list)          # without memory of a plan's own
+    where.sync()
+    assert torch.equal(got, again) and torch.equal(got, once) and got.shape == (1,) and got.dtype == torch.float32
 
 
 @pytest.mark.parametrize("dtype", ["f32", "bf16"])
@@ -943,6 +945,9 @@ def test_refusals_of_blocks_and_norm(cpu):
         optim.grad_norm([x], out=torch.zeros(2))
     with pytest.raises(RuntimeError, match="contiguous"):
         optim.grad_norm([torch.zeros(4, 4).t()])
+    for i in (0, 150, 299):
+        with pytest.raises(_native.NativeError, match="overlap"):
+            optim.grad_norm([x[:200], x, x[10:20]], out=x[i:i + 1])
 
 
 def test_tensors_on_the_cpu_are_refused():
@@ -978,7 +983,7 @@ def test_c_entries_refuse_with_a_code_and_a_message():
     assert raw.pccl_optim_plan_norm(None, None, None, None, 0) == -1
     assert raw.pccl_optim_plan_norm(ctypes.byref(h), None, None, None, -1) == -1 and not h
     assert raw.pccl_optim_plan_norm(ctypes.byref(h), None, None, None, 1) == -1 and not h
-    assert raw.pccl_optim_run_norm(None, None, None, 0, None) == -1
+    assert raw.pccl_optim_run_norm(None, None, None, 0, None, None) == -1
     assert raw.pccl_optim_run_blocks(None, None) == -1
     assert raw.pccl_optim_run_adamw(None, None, None, None, None) == -1
     assert raw.pccl_optim_table_fill(None, None, 0) == -1 and raw.pccl_optim_table_bytes(None) == 0
@@ -988,9 +993,12 @@ def test_c_entries_refuse_with_a_code_and_a_message():
     with pytest.raises(E, match="another operator"):
         lib.run_blocks(norm)
     with pytest.raises(E, match="bytes of work space"):
-        lib.run_norm(norm, 64, 0, 0)
+        lib.run_norm(norm, 1 << 30, 0, 0)
     with pytest.raises(E, match="out is NULL"):
-        lib.run_norm(norm, 0, 64, 1 << 20)
+        lib.run_norm(norm, 0, 1 << 30, 1 << 20)
+    for out, work, ticket in ((64, 1 << 30, 0), (1 << 30, 64 + (1 << 22) - 8, 0), (1 << 30, 1 << 31, 128)):
+        with pytest.raises(E, match="overlap"):
+            lib.run_norm(norm, out, work, 1 << 20, ticket)
     step = lib.plan_adamw([64], [128], [192], [256], None, [4], [0], [0], None)
     s = _optim_native.Step(lr=1e-3, beta1=0.9, beta2=0.99, eps=1e-8, grad_scale=1.0, step=1)
     with pytest.raises(E, match=r"grads\[0\] is NULL"):
@@ -1172,7 +1180,7 @@ def test_a_plan_of_many_tensors_on_other_streams_and_in_a_graph_that_outlives_it
         return s, (optim.plan_adamw8 if eight else optim.plan_adamw)(*(s[k].list for k in keys), **HYPER)
     a, plan_a = fresh()
     b, plan_b = fresh()
-    assert plan_a._table is not None
+    assert plan_a._own is not None
     side = torch.cuda.Stream()
     torch.cuda.synchronize()
     plan_a(1)
