@@ -23,7 +23,7 @@ def compile_library(force: bool = False, verbose: bool = False) -> str:
     """Run the Makefile in csrc/ (hipcc cross-compiles gfx950 without a GPU)."""
     if shutil.which("make") is None:
         raise RuntimeError("cannot build libpccl_hip.so: `make` not found")
-    cmd = ["make", "-C", CSRC_DIR] + (["-B"] if force else [])
+    cmd = ["make", "-j2", "-C", CSRC_DIR] + (["-B"] if force else [])
     proc = subprocess.run(cmd, capture_output=True, text=True)
     if verbose or proc.returncode:
         print(proc.stdout)

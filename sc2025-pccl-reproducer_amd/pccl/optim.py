@@ -59,17 +59,15 @@ def _check_list(what, name, tensors, like=None, dtype=None):
         like = tensors
     if len(tensors) != len(like):
         raise ValueError(f"{what}: need one {name} tensor per entry of the first list ({len(like)}), got {len(tensors)}")
-    device = None
+    gpu = like[0].get_device() if like else -1
     for i, (t, p) in enumerate(zip(tensors, like)):
         kernels.check_device_tensor(t, name)
         if dtype is not None and t.dtype != dtype:
             raise RuntimeError(f"{what}: {name}[{i}] must be of type {dtype}, got {t.dtype}")
-        if t.shape != p.shape and (t.numel() != p.numel() or (t.dim() > 1 and p.dim() > 1)):
+        if t is not p and t.shape != p.shape and (t.numel() != p.numel() or (t.dim() > 1 and p.dim() > 1)):
             raise RuntimeError(f"{what}: {name}[{i}] has shape {tuple(t.shape)}, its partner {tuple(p.shape)}")
-        if device is None:
-            device = like[0].device
-        if t.device != device:
-            _check_device(what, f"{name}[{i}]", t, device)
+        if t.get_device() != gpu:
+            _check_device(what, f"{name}[{i}]", t, like[0].device)
     return tensors
 
 
@@ -86,7 +84,8 @@ def _check_scales(what, name, scales, codes):
         kernels.check_device_tensor(s, f"{name}[{i}]")
         if s.dtype != torch.float32 or s.numel() != block_count(c.numel()):
             raise RuntimeError(f"{what}: {name}[{i}] must hold {block_count(c.numel())} float32 scales (one per {BLOCK} elements)")
-        _check_device(what, f"{name}[{i}]", s, c.device)
+        if s.get_device() != c.get_device():
+            _check_device(what, f"{name}[{i}]", s, c.device)
     return scales
 
 
@@ -116,9 +115,9 @@ def _capturing(index):
 
 
 def _hold(*lists):
-    """Aliases of the tensors: their memory lives as long as the plan, also when
-    a tensor object is given other storage."""
-    return [t.detach() for ts in lists if ts is not None for t in ts if t is not None]
+    """The memory of the tensors: it lives as long as the plan, also when a tensor
+    object is given other storage."""
+    return [t.untyped_storage() for ts in lists if ts is not None for t in ts if t is not None]
 
 
 class _Plan:
