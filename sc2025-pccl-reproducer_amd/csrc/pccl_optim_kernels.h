@@ -507,6 +507,9 @@ struct Hyper {
   const float* norm;
 };
 
+static_assert(sizeof(AdamTable) + sizeof(Hyper) + 16 <= 4096 && sizeof(Adam8Table) + sizeof(Hyper) + 16 <= 4096 &&
+              sizeof(BlocksTable) + 16 <= 4096 && sizeof(NormTable) + 48 <= 4096, "kernel arguments");
+
 // base^n by squaring: the error is n roundings of 2^-53 at most, and n base^n is bounded
 __device__ __forceinline__ double int_power(double base, uint64_t n) {
   double r = 1.0;

@@ -34,6 +34,7 @@ from ._optim_native import BLOCK, TICKET_BYTES, Step
 CODE_DTYPE = torch.float8_e4m3fn      # of the 8-bit codes
 
 _increment_version = torch.autograd.graph.increment_version
+_current_device = kernels._current_device or torch.cuda.current_device
 
 
 def block_count(numel: int) -> int:
@@ -129,7 +130,7 @@ class _Plan:
 
     def _on_device(self, fn, *args):
         """fn(*args, stream) on the current stream of the tensors' device, whatever the current device is."""
-        if self._index is None or self._index == kernels._current_device():
+        if self._index is None or self._index == _current_device():
             return fn(*args, kernels.stream_handle())
         with torch.cuda.device(self._index):
             return fn(*args, kernels.stream_handle())
@@ -147,10 +148,10 @@ class _Plan:
     _own = _own_stream = None
 
     def _make_own(self, make):
-        if not _capturing(self._index):
-            def put(stream):
+        def put(stream):
+            if not _capturing(self._index):
                 self._own, self._own_stream = make(), stream
-            self._on_device(put)
+        self._on_device(put)
 
     def _usable(self, stream):
         return self._own is not None and stream == self._own_stream and not _capturing(self._index)
@@ -168,7 +169,8 @@ class AdamWPlan(_Plan):
         self._like = [(g.numel(), g.shape, g.dtype) for g in grads]      # for calls that bring other gradients
         self._base = Step(beta1=betas[0], beta2=betas[1], eps=eps, weight_decay=weight_decay, grad_scale=1.0)
         self._set_lr(self._base, lr)
-        self._keep.append(lr)
+        if isinstance(lr, torch.Tensor):
+            self._keep += _hold([lr])
         if table:
             self._make_table()
 
@@ -271,7 +273,7 @@ def plan_adamw(params: Sequence[torch.Tensor], grads: Sequence[torch.Tensor], ex
                exp_avg_sq: Sequence[torch.Tensor], *, copies: Optional[Sequence[Optional[torch.Tensor]]] = None,
                lr: Union[float, torch.Tensor] = 1e-3, betas: Tuple[float, float] = (0.9, 0.999), eps: float = 1e-8,
                weight_decay: float = 1e-2) -> AdamWPlan:
-    """AdamW over many tensors in one launch per 64 of them, moments in float32.
+    """AdamW over many tensors, in one launch for up to 4096 of the same types, moments in float32.
 
     params   float32, bfloat16 or float16, updated in place in their own type
     grads    of any of these types, read only
@@ -283,6 +285,7 @@ def plan_adamw(params: Sequence[torch.Tensor], grads: Sequence[torch.Tensor], ex
 
     step        1 for the first step; or a one-element int64 tensor on the GPU
     grads       other gradients than the plan's, of the same types and shapes
+                (a loop whose gradients are new tensors at every step passes them here)
     lr          another learning rate; or a one-element float32 tensor on the GPU
     grad_scale  factor of all gradients (1 / loss scale, 1 / ranks)
     norm, max_norm    the result of grad_norm over the gradients as they are
