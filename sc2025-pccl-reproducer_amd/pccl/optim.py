@@ -185,10 +185,13 @@ class AdamWPlan(_Plan):
         size = self._lib.table_bytes(self._native)
         if not size:
             return
-        pinned = self._index is not None
-        host = torch.empty(size, dtype=torch.uint8, pin_memory=pinned)
-        self._lib.table_fill(self._native, host.data_ptr(), size)
-        self._make_own(lambda: host.to(self._device, non_blocking=True) if pinned else host)
+
+        def make():
+            pinned = self._index is not None
+            host = torch.empty(size, dtype=torch.uint8, pin_memory=pinned)
+            self._lib.table_fill(self._native, host.data_ptr(), size)
+            return host.to(self._device, non_blocking=True) if pinned else host
+        self._make_own(make)
 
     def _step(self, grads, s, stream):
         table = self._own.data_ptr() if grads is None and self._usable(stream) else None

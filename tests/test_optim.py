@@ -1202,6 +1202,34 @@ def test_a_plan_of_many_tensors_on_other_streams_and_in_a_graph_that_outlives_it
 
 
 @pytest.mark.gpu
+def test_plans_made_and_single_calls_made_during_capture():
+    """Neither allocates host memory, copies or clears anything while a graph is captured."""
+    from pccl import optim
+    dev, sizes = "cuda:0", [2000 + k for k in range(70)]
+    a, b = (make(sizes, dev, seed=65, c="bf16") for _ in range(2))
+    norm = torch.zeros(1, device=dev)
+
+    def body(s):
+        optim.plan_grad_norm(s["g"].list)(norm)
+        optim.plan_adamw(s["p"].list, s["g"].list, s["m"].list, s["v"].list, copies=s["c"].list, **HYPER)(
+            2, norm=norm, max_norm=0.1)
+        optim.adamw(s["p"].list, s["g"].list, s["m"].list, s["v"].list, 3, copies=s["c"].list, norm=optim.grad_norm(s["g"].list),
+                    max_norm=0.1, **HYPER)
+    body(a)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        body(b)
+    for _ in range(3):
+        graph.replay()
+        torch.cuda.synchronize()
+        for k in ("p", "m", "v", "c"):
+            assert np.array_equal(Flat.raw(a[k].flat), Flat.raw(b[k].flat)), k
+        body(a)
+        torch.cuda.synchronize()
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("eight", [False, True])
 def test_adamw_offsets_beyond_32_bits(eight):
     """A tensor of more than 2^32 elements, zero but for a few: they are stepped, and nothing else is."""
