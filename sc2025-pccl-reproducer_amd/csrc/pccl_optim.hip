@@ -346,13 +346,16 @@ int make_adamw(pccl_optim_plan& plan, Checker& check, void* const* params, const
 
 int make_hyper(const pccl_optim_plan& plan, const pccl_optim_step& s, Hyper& h, const char* what) {
   auto bad = [&](const char* name, double x) { return fail(PCCL_HIP_EINVAL, "%s: %s = %g is not allowed", what, name, x); };
-  if (!(s.lr >= 0) || !std::isfinite(s.lr)) return bad("lr", s.lr);
+  // what the kernels hold in fp32 is checked as that: 0 there means something else, and infinity gives NaN
+  auto fits = [](double x) { return std::isfinite((float)x); };
+  if (!(s.lr >= 0) || !fits(s.lr)) return bad("lr", s.lr);
   if (!(s.beta1 >= 0 && s.beta1 < 1)) return bad("beta1", s.beta1);
   if (!(s.beta2 >= 0 && s.beta2 < 1)) return bad("beta2", s.beta2);
-  if (!(s.eps >= 0) || !std::isfinite(s.eps) || (s.eps > 0 && s.eps < 0x1p-126)) return bad("eps", s.eps);
+  if (!(s.eps >= 0) || !fits(s.eps) || (s.eps > 0 && s.eps < 0x1p-126)) return bad("eps", s.eps);
   if (!(s.weight_decay >= 0) || !std::isfinite(s.weight_decay)) return bad("weight_decay", s.weight_decay);
-  if (!std::isfinite(s.grad_scale) || (float)s.grad_scale == 0.0f || std::isinf((float)s.grad_scale)) return bad("grad_scale", s.grad_scale);
-  if (!(s.max_norm >= 0) || !std::isfinite(s.max_norm)) return bad("max_norm", s.max_norm);
+  if (!s.lr_dev && !fits(s.lr * s.weight_decay)) return bad("lr * weight_decay", s.lr * s.weight_decay);
+  if (!fits(s.grad_scale) || (float)s.grad_scale == 0.0f) return bad("grad_scale", s.grad_scale);
+  if (!(s.max_norm >= 0) || !fits(s.max_norm) || (s.max_norm > 0 && (float)s.max_norm == 0.0f)) return bad("max_norm", s.max_norm);
   if (s.max_norm > 0 && !s.norm) return fail(PCCL_HIP_EINVAL, "%s: max_norm without a norm", what);
   if (s.skip_nonfinite && !s.norm) return fail(PCCL_HIP_EINVAL, "%s: skip_nonfinite without a norm", what);
   if (!s.step_dev && s.step < 1) return fail(PCCL_HIP_EINVAL, "%s: step %lld: the first step is 1", what, (long long)s.step);
@@ -384,7 +387,9 @@ int make_hyper(const pccl_optim_plan& plan, const pccl_optim_step& s, Hyper& h, 
   h.step_dev = s.step_dev;
   h.norm = s.norm;
   h.lr_decay = (float)(s.lr * s.weight_decay);
-  h.step_size = (float)(s.lr / (1.0 - std::pow(s.beta1, (double)h.step)));
+  const double step_size = s.lr / (1.0 - std::pow(s.beta1, (double)h.step));
+  if (!s.lr_dev && !s.step_dev && !fits(step_size)) return bad("lr / (1 - beta1^step)", step_size);
+  h.step_size = (float)step_size;
   h.inv_root_bias = (float)(1.0 / std::sqrt(1.0 - std::pow(s.beta2, (double)h.step)));
   return PCCL_HIP_OK;
 }
