@@ -406,11 +406,20 @@ __device__ __forceinline__ uint32_t noise(uint32_t key, size_t first, uint32_t i
   return mix32((uint32_t)first + key + (uint32_t)((uint64_t)first >> 32) * 0x9e3779b1u + i);
 }
 
-// The scale of a block and its reciprocal, in two parts: inv is good to a unit in
-// the last place, rest is what is missing.
-struct BlockScale { float scale, inv, rest; };
+struct BlockScale { float scale, inv; };
 constexpr float kInvCodeMax = 1.0f / kCodeMax;
 constexpr uint32_t kInfBits = 0x7f800000u;
+
+// 1 / x for a normal x whose reciprocal is normal: the hardware's, good to one
+// unit in the last place, and one Newton step, which makes it the rounded one.
+__device__ __forceinline__ float reciprocal(float x) {
+#if defined(__HIP_DEVICE_COMPILE__)
+  const float r = __builtin_amdgcn_rcpf(x);
+  return __builtin_fmaf(__builtin_fmaf(-x, r, 1.0f), r, r);
+#else
+  return 1.0f / x;
+#endif
+}
 
 // From the largest |x| of a block, as bits.  The comparisons are of integers, in
 // which NaN is above infinity, so that either becomes the scale.  a / 448 by the
@@ -423,22 +432,9 @@ __device__ __forceinline__ BlockScale block_scale(uint32_t amax_bits) {
   BlockScale s;
   const float a = __uint_as_float(amax_bits > kFloorBits ? amax_bits : kFloorBits), near = a * kInvCodeMax;
   s.scale = amax_bits < kInfBits ? __builtin_fmaf(__builtin_fmaf(-near, kCodeMax, a), kInvCodeMax, near) : near;
-#if defined(__HIP_DEVICE_COMPILE__)
-  s.inv = __builtin_amdgcn_rcpf(s.scale);
-#else
-  s.inv = 1.0f / s.scale;
-#endif
-  s.rest = __builtin_fmaf(-s.scale, s.inv, 1.0f) * s.inv;
+  s.inv = reciprocal(s.scale);
   return s;
 }
-
-// x / scale, rounded once: the two parts together are good to 2^-46, so a quotient
-// that is a code or half way between two comes out as that (every mantissa of the
-// scale was tried with every such quotient).  The product with one rounded
-// reciprocal misses 10 % of those quotients by a unit, and 16-bit data, whose
-// scales have few bits, is full of them.  The product more costs k_quantize 0.5 us
-// in 64 (128 Mi bf16 elements) and k_adamw8 nothing that shows.
-__device__ __forceinline__ float over_scale(float x, const BlockScale& s) { return __builtin_fmaf(x, s.inv, x * s.rest); }
 
 __device__ __forceinline__ uint32_t amax4(const float* x) {
   uint32_t a = 0;
@@ -710,8 +706,8 @@ __global__ __launch_bounds__(kWave) void k_adamw8(Adam8Table args, const void* d
         uint32_t yc, zc;
 #pragma unroll
         for (int e = 0; e < kVec; ++e) {
-          y[e] = over_scale(m[k][e], mb);
-          z[e] = lift_root(r[k][e], over_scale(r[k][e], rb));
+          y[e] = m[k][e] * mb.inv;
+          z[e] = lift_root(r[k][e], r[k][e] * rb.inv);
         }
         if (h.stochastic) {
           uint32_t yb[kVec], zb[kVec];
@@ -777,7 +773,7 @@ __global__ __launch_bounds__(kWave) void k_quantize(BlocksTable args, int count,
         float y[kVec];
 #pragma unroll
         for (int e = 0; e < kVec; ++e) {
-          y[e] = over_scale(x[k][e], b);
+          y[e] = x[k][e] * b.inv;
           if (root) y[e] = lift_root(x[k][e], y[e]);
         }
         store_codes<NT, FULL>(codes, u * kBlock + lane * kVec, span, encode4(y));

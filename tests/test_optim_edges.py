@@ -71,74 +71,6 @@ def test_codes_of_a_block_whose_scale_is_exact(where):
     assert float(scales) == 3.5 and codes.float().cpu().tolist() == [448.0, 1.25, 1.5, -1.25]
 
 
-def codes_and_ties():
-    """Every finite code of either sign and every value half way between two of them, and the codes these belong to."""
-    code = torch.arange(127, dtype=torch.uint8).view(torch.float8_e4m3fn).float()
-    t = torch.cat([code, (code[1:] + code[:-1]) / 2])
-    t = torch.cat([t, -t[1:]])
-    return t, t.to(torch.float8_e4m3fn).float()
-
-
-def exact_scale_blocks(dtype):
-    """Blocks whose scale is s = k 2^j, with elements t * s, t a code or a tie: all of them numbers of the type."""
-    t, want = codes_and_ties()
-    widest, low, high = {"f32": (1 << 18, -60, 50), "bf16": (32, -60, 50), "f16": (128, -10, 1)}[dtype]
-    rng = np.random.default_rng(7)
-    ks = np.arange(1, 128, 2) if dtype != "f32" else np.concatenate([np.arange(1, 512, 2), rng.integers(256, widest, 500) * 2 + 1])
-    x, w, s = [], [], []
-    for k in ks:
-        if k >= widest:
-            continue
-        scale = float(k) * 2.0 ** int(rng.integers(low, high - int(k).bit_length() + 1))
-        for part in range(0, t.numel(), BLOCK - 1):
-            tt, ww = t[part:part + BLOCK - 1], want[part:part + BLOCK - 1]
-            xx = tt.double() * scale
-            fits = xx.to(TYPES[dtype]).double() == xx
-            xx, ww = torch.where(fits, xx, torch.zeros(())), torch.where(fits, ww, torch.zeros(()))
-            x.append(torch.nn.functional.pad(torch.cat([torch.tensor([448.0 * scale], dtype=torch.float64), xx]), (0, BLOCK - 1 - tt.numel())))
-            w.append(torch.nn.functional.pad(torch.cat([torch.tensor([448.0]), ww]), (0, BLOCK - 1 - tt.numel())))
-            s.append(scale)
-    x = torch.cat(x)
-    assert torch.equal(x.to(TYPES[dtype]).double(), x)
-    return x.to(TYPES[dtype]), torch.cat(w), fp32(s)
-
-
-@pytest.mark.parametrize("dtype", ["f32", "bf16", "f16"])
-def test_codes_and_ties_of_blocks_whose_scale_is_exact(where, dtype):
-    """x / scale is a code or a tie without any rounding: the code is that one, or the even one."""
-    from pccl import optim
-    x, want, s = exact_scale_blocks(dtype)
-    x = x.to(where.device)
-    codes, scales = optim.empty_blocks(x)
-    optim.quantize_blocks([codes], [scales], [x])
-    where.sync()
-    assert np.array_equal(scales.cpu().numpy(), s)
-    got = codes.float().cpu()
-    bad = (got != want).nonzero().reshape(-1)
-    assert not bad.numel(), (bad.numel(), [(float(x[i]), float(s[i // BLOCK]), float(got[i]), float(want[i])) for i in bad[:4].tolist()])
-
-
-@pytest.mark.parametrize("dtype", ["f32", "bf16", "f16"])
-def test_moments_on_codes_and_ties(where, dtype):
-    """With both betas 0 the new first moment is the gradient: to nearest the codes are those of quantize_blocks, and a
-    gradient that is a code times its scale stays that code whatever the random bits."""
-    from pccl import optim
-    g, want, s = exact_scale_blocks(dtype)
-    t, w = codes_and_ties()
-    is_code = torch.isin(want, t[t == w]) & (g.double() == want.double() * torch.from_numpy(s).double().repeat_interleave(BLOCK))
-    g = g.to(where.device)
-    for seed in (None, 0, 1, 2):
-        p = torch.zeros(g.numel(), device=where.device)
-        m, ms = optim.empty_blocks(p)
-        r, rs = optim.empty_blocks(p)
-        optim.adamw8([p], [g], [m], [r], [ms], [rs], 1, betas=(0.0, 0.0), weight_decay=0.0, seed=seed)
-        where.sync()
-        assert np.array_equal(ms.cpu().numpy(), s)
-        got = m.float().cpu()
-        ok = (got == want) if seed is None else (got == want) | ~is_code
-        assert ok.all(), (seed, int((~ok).sum()))
-
-
 # ---------------------------------------------------------------------------
 # scalars
 # ---------------------------------------------------------------------------
