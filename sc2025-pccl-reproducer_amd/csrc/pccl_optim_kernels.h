@@ -407,8 +407,7 @@ __device__ __forceinline__ uint32_t noise(uint32_t key, size_t first, uint32_t i
 }
 
 struct BlockScale { float scale, inv; };
-constexpr float kInvCodeMax = 1.0f / kCodeMax;
-constexpr uint32_t kInfBits = 0x7f800000u;
+constexpr float kInvCodeMax = 1.0f / kCodeMax;   // 448 times it is exactly 1
 
 // 1 / x for a normal x whose reciprocal is normal: the hardware's, good to one
 // unit in the last place, and one Newton step, which makes it the rounded one.
@@ -421,17 +420,11 @@ __device__ __forceinline__ float reciprocal(float x) {
 #endif
 }
 
-// From the largest |x| of a block, as bits.  The comparisons are of integers, in
-// which NaN is above infinity, so that either becomes the scale.  a / 448 by the
-// product with 1 / 448, which alone is one unit off for 55 % of all a, and a
-// correction by the exact residue: the rounded quotient for every mantissa (all
-// 2^23 were compared, at exponents from the floor's to the largest), without the
-// ten instructions of a division.  A scale that is off by a unit moves values
-// across the borders between codes, in all of its block.
+// From the largest |x| of a block, as bits.  The comparison is one of integers,
+// in which NaN is above infinity, so that either becomes the scale.
 __device__ __forceinline__ BlockScale block_scale(uint32_t amax_bits) {
   BlockScale s;
-  const float a = __uint_as_float(amax_bits > kFloorBits ? amax_bits : kFloorBits), near = a * kInvCodeMax;
-  s.scale = amax_bits < kInfBits ? __builtin_fmaf(__builtin_fmaf(-near, kCodeMax, a), kInvCodeMax, near) : near;
+  s.scale = __uint_as_float(amax_bits > kFloorBits ? amax_bits : kFloorBits) * kInvCodeMax;
   s.inv = reciprocal(s.scale);
   return s;
 }
