@@ -133,10 +133,14 @@ int pccl_optim_run_norm(const pccl_optim_plan* plan, float* out, void* work, siz
 
 /* ---- 8-bit blocks --------------------------------------------------------
  * Blocks of 256 consecutive elements from the start of each tensor, the last
- * one possibly shorter.  With a the largest |x| of a block:
+ * one possibly shorter.  With a the largest |x| of a block, every operation in
+ * fp32 and rounded by itself:
  *
- *   scale = max(a, 2^-100) / 448      code = e4m3(x / scale), to nearest, ties to even
+ *   scale = max(a, 2^-100) * (1 / 448)      code = e4m3(x * (1 / scale)), to nearest, ties to even
  *
+ * (what elementary operations that divide by a multiplication with the reciprocal
+ * give, bit for bit).  The products are within 2^-22 of the quotients: of a value
+ * that is so near to the middle between two codes either neighbour may be taken.
  * root = 1 (x >= 0, second moments) holds sqrt(x) in place of x and gives a
  * value other than 0 at least the smallest code, 2^-9, so that it is not read
  * back as 0.  Read back: code * scale, or its square.  Inf or NaN in a block

@@ -427,9 +427,10 @@ def plan_quantize_blocks(codes: Sequence[torch.Tensor], scales: Sequence[torch.T
                          root: bool = False) -> BlocksPlan:
     """Tensors to float8_e4m3fn codes with one float32 scale per 256 elements.
 
-    With a the largest magnitude of a block: scale = max(a, 2**-100) / 448, code
-    = the e4m3 value nearest to x / scale, so x is off by at most 2**-4 of itself
-    or 2**-10 of the scale.  root=True is for second moments (x >= 0): the codes
+    With a the largest magnitude of a block: scale = max(a, 2**-100) * (1 / 448),
+    code = the e4m3 value nearest to x * (1 / scale), each operation rounded to
+    float32, so x is off by at most 2**-4 of itself or 2**-10 of the scale (and by
+    the roundings, 2**-22).  root=True is for second moments (x >= 0): the codes
     hold sqrt(x), and no x but 0 gets the code 0.  An inf or NaN spoils its whole
     block.  Codes and scales of the ranks' shards can be gathered like any other
     tensors (for that, let shards be multiples of 256)."""

@@ -13,6 +13,10 @@ from optim_oracle import BLOCK, TYPES, f64
 from test_optim import (HYPER, Flat, check_adamw, check_adamw8, cpu, make, values, values8, where)  # noqa: F401 - fixtures
 
 
+def fp32(x):
+    return np.asarray(x, np.float32)
+
+
 # ---------------------------------------------------------------------------
 # scalars
 # ---------------------------------------------------------------------------
@@ -48,3 +52,68 @@ def test_the_smallest_and_largest_norm_to_clip_to(where, max_norm):
     where.sync()
     # the clip factor is a denormal of one bit and its neighbours: off by half of 2^-149, a gradient below 1e-2 with it
     check_adamw(s, old, 3, "clip", norm=10.0, max_norm=max_norm, **HYPER)
+
+
+# ---------------------------------------------------------------------------
+# the 8-bit form, bit for bit
+# ---------------------------------------------------------------------------
+
+def plain_codes(x, root=False, u16=None):
+    """(codes, scales) of fp32 values in elementary fp32 operations, each rounded by itself: scale = max(a, 2^-100) * (1/448),
+    code = e4m3(x * (1 / scale)).  u16: 16 random bits per value, added below the mantissa bits that e4m3 keeps."""
+    one, n = fp32(1), x.size
+    x = np.pad(x, (0, -n % BLOCK)).reshape(-1, BLOCK)
+    scale = np.maximum(np.abs(x).max(1), fp32(2.0 ** -100)) * (one / fp32(448))
+    y = x * (one / scale)[:, None]
+    if root:
+        y = np.where((x != 0) & (y < fp32(2.0 ** -9)), fp32(2.0 ** -9), y)
+    if u16 is not None:
+        u16 = np.pad(u16.astype(np.uint32), (0, -n % BLOCK)).reshape(-1, BLOCK)
+        a = np.minimum(np.abs(y), fp32(448))
+        shift = np.where(a < fp32(2.0 ** -6), fp32(2.0 ** -6), fp32(0))        # subnormal codes are as far apart as those from 2^-6 on
+        cut = (((a + shift).view(np.uint32) + (u16 << 4)) & np.uint32(0xfff00000)).view(np.float32) - shift
+        y = np.copysign(cut, y)
+    assert y.dtype == np.float32 and scale.dtype == np.float32
+    y = torch.from_numpy(np.clip(y, -448, 448).reshape(-1)[:n].copy()).to(torch.float8_e4m3fn)
+    return y.view(torch.uint8).numpy(), scale
+
+
+def read(codes, scales):
+    """code * scale, rounded to fp32."""
+    return codes.float().cpu().numpy() * np.repeat(scales.cpu().numpy(), BLOCK)[:codes.numel()]
+
+
+def block_values(dtype, where, root):
+    """Values of all magnitudes and, in every second block, ones that lie on codes and half way between them."""
+    blocks = 4000 if where.name == "hip" else 400
+    rng = np.random.default_rng(101)
+    x = rng.standard_normal((blocks, BLOCK)) * 10.0 ** rng.uniform(-4, 0, (blocks, BLOCK))
+    step = rng.integers(1, 32, (blocks, 1)) * 2.0 ** rng.integers(-6, 3, (blocks, 1))
+    x[::2] = (step * rng.integers(-255, 256, (blocks, BLOCK)) / 8)[::2]
+    x[::2, 0] = (step * 56)[::2, 0]
+    if dtype == "f32":
+        x *= 2.0 ** rng.integers(-95, 110, (blocks, 1)) if not root else 2.0 ** rng.integers(-40, 50, (blocks, 1))
+        x[1], x[3], x[5, 0] = 0, 1e-45, np.finfo(np.float32).max if not root else 2.0 ** 60
+    x = torch.from_numpy(x.reshape(-1)[:-100]).to(TYPES[dtype])
+    return (x.float() * x.float()).to(TYPES[dtype]) if root else x
+
+
+@pytest.mark.parametrize("root", [False, True])
+@pytest.mark.parametrize("dtype", ["f32", "bf16", "f16"])
+def test_blocks_are_those_of_elementary_fp32_operations(where, dtype, root):
+    from pccl import optim
+    x = block_values(dtype, where, root).to(where.device)
+    codes, scales = optim.empty_blocks(x)
+    optim.quantize_blocks([codes], [scales], [x], root=root)
+    back = torch.empty(x.shape, device=where.device)
+    optim.dequantize_blocks([back], [codes], [scales], root=root)
+    where.sync()
+    v = x.float().cpu().numpy()
+    with np.errstate(invalid="ignore"):
+        want_codes, want_scales = plain_codes(np.sqrt(v) if root else v, root)
+        r = read(codes, scales)
+    assert np.array_equal(scales.cpu().numpy(), want_scales)
+    got, back = codes.view(torch.uint8).cpu().numpy(), back.cpu().numpy()
+    fine = np.repeat(np.isfinite(want_scales), BLOCK)[:got.size]      # squares beyond float16: the codes of such a block are open
+    assert np.array_equal(got[fine], want_codes[fine]), np.flatnonzero((got != want_codes) & fine)[:5]
+    assert np.array_equal(back[fine], (r * r if root else r)[fine]) and not np.isfinite(back[~fine]).any()
