@@ -456,19 +456,21 @@ __device__ __forceinline__ float lift_root(float r, float y) {
 #endif
 }
 
-// sqrt of four numbers >= 0.  For normal ones from the hardware's 1 / sqrt(x),
-// good to one unit in the last place, and a correction by the exact residue, a
-// third of the instructions of sqrtf: correctly rounded in all but about one of
-// a million cases.  Zeros, denormals, infinity and NaN go the long way.
+// sqrt of four numbers >= 0.  From 2^-102 on from the hardware's 1 / sqrt(x), good
+// to one unit in the last place, and a correction by the exact residue, a third of
+// the instructions of sqrtf: the rounded root for every such number (all were
+// compared on MI355X).  Below that the residue underflows, and the root would be one
+// unit off for up to 9 % of a binade; they, zeros, infinity and NaN go the long way.
+constexpr uint32_t kRootFrom = 0x0c800000u;      // 2^-102
 __device__ __forceinline__ void sqrt4(const float* x, float* root) {
 #if defined(__HIP_DEVICE_COMPILE__)
   uint32_t top = 0;
 #pragma unroll
   for (int e = 0; e < kVec; ++e) {
-    const uint32_t b = __float_as_uint(x[e]) - 0x00800000u;      // below 0x7f000000 for the normal ones alone
+    const uint32_t b = __float_as_uint(x[e]) - kRootFrom;      // wraps for those below
     top = b > top ? b : top;
   }
-  if (top < 0x7f000000u) {
+  if (top < 0x7f800000u - kRootFrom) {
 #pragma unroll
     for (int e = 0; e < kVec; ++e) {
       const float r = __builtin_amdgcn_rsqf(x[e]);

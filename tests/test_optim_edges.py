@@ -117,3 +117,35 @@ def test_blocks_are_those_of_elementary_fp32_operations(where, dtype, root):
     fine = np.repeat(np.isfinite(want_scales), BLOCK)[:got.size]      # squares beyond float16: the codes of such a block are open
     assert np.array_equal(got[fine], want_codes[fine]), np.flatnonzero((got != want_codes) & fine)[:5]
     assert np.array_equal(back[fine], (r * r if root else r)[fine]) and not np.isfinite(back[~fine]).any()
+
+
+@pytest.mark.parametrize("seed", [None, 0, 4000000000])
+@pytest.mark.parametrize("g", ["f32", "bf16", "f16"])
+def test_moments_are_those_of_elementary_fp32_operations(where, g, seed):
+    """Both moments of two steps, to nearest and with random bits, clipped by a norm, at a grad_scale that is a power of two."""
+    from pccl import optim
+    b1, b2 = 0.9, 0.99
+    grad = (block_values(g, where, False).float() * 2.0 ** -4).to(TYPES[g])
+    grad = torch.where(grad.float().abs() < 1e15, grad, torch.zeros_like(grad)).to(where.device)
+    p = torch.zeros(grad.numel(), device=where.device)
+    m, ms = optim.empty_blocks(p)
+    r, rs = optim.empty_blocks(p)
+    norm = torch.tensor([2.5 * 1024], device=where.device)
+    plan = optim.plan_adamw8([p], [grad], [m], [r], [ms], [rs], betas=(b1, b2))
+    # max_norm / (norm * grad_scale + 1e-6), then times grad_scale, then times the gradient
+    factor = fp32(1) / (fp32(2.5) + fp32(1e-6)) * fp32(2.0 ** -10)
+    gs = grad.float().cpu().numpy() * factor
+    for step in (1, 2):
+        old_m, old_r = read(m, ms), read(r, rs)
+        plan(step, seed=seed, norm=norm, max_norm=1.0, grad_scale=2.0 ** -10)
+        where.sync()
+        new_m = fp32(b1) * old_m + fp32(1 - b1) * gs
+        new_r = np.sqrt(fp32(b2) * (old_r * old_r) + fp32(1 - b2) * (gs * gs))
+        assert new_m.dtype == new_r.dtype == np.float32
+        bits = None if seed is None else Q.noise(seed, step, p.numel())
+        for name, codes, scales, x, root, u in (("m", m, ms, new_m, False, None if bits is None else bits & np.uint64(0xffff)),
+                                                ("r", r, rs, new_r, True, None if bits is None else bits >> np.uint64(16))):
+            want_codes, want_scales = plain_codes(x, root, u)
+            assert np.array_equal(scales.cpu().numpy(), want_scales), (name, step)
+            got = codes.view(torch.uint8).cpu().numpy()
+            assert np.array_equal(got, want_codes), (name, step, np.flatnonzero(got != want_codes)[:5])
