@@ -375,6 +375,9 @@ int make_hyper(const pccl_optim_plan& plan, const pccl_optim_step& s, Hyper& h, 
   h.eps = (float)s.eps;
   h.grad_scale = (float)s.grad_scale;
   h.max_norm = (float)s.max_norm;
+  h.scale_high = std::max(1.0f, std::fabs(h.grad_scale));
+  h.scale_low = h.grad_scale / h.scale_high;
+  h.norm_added = 1e-6f / h.scale_high;
   h.skip_nonfinite = s.skip_nonfinite != 0;
   h.stochastic = s.stochastic != 0;
   h.seed = s.seed;

@@ -504,6 +504,8 @@ template <bool NT, bool FULL> __device__ __forceinline__ uint32_t load_codes(cgp
 struct Hyper {
   float beta1, one_minus_beta1, beta2, one_minus_beta2, eps;
   float grad_scale, max_norm;
+  float scale_high, scale_low;   // grad_scale as max(1, |grad_scale|) times what is left: one of them is 1 or -1
+  float norm_added;              // 1e-6 / scale_high
   float lr_decay;        // lr * weight_decay
   float step_size;       // lr / (1 - beta1^t)
   float inv_root_bias;   // 1 / sqrt(1 - beta2^t)
@@ -542,8 +544,10 @@ __device__ __forceinline__ bool finish_hyper(Hyper& h) {
     const float norm = *(const PCCL_GLOBAL float*)(uintptr_t)h.norm;
     if (h.skip_nonfinite && !(std::fabs(norm) <= 3.402823466e38f)) return false;
     if (h.max_norm > 0.0f) {
-      const float c = h.max_norm / (norm * std::fabs(h.grad_scale) + 1e-6f);
-      h.grad_scale *= c >= 1.0f ? 1.0f : c;      // a NaN norm gives NaN gradients
+      // grad_scale * min(1, max_norm / (norm * |grad_scale| + 1e-6)), with a grad_scale above 1 taken into the
+      // fraction: norm * grad_scale may overflow where the result does not.
+      const float c = h.max_norm / (norm * std::fabs(h.scale_low) + h.norm_added);
+      h.grad_scale = h.scale_low * (c >= h.scale_high ? h.scale_high : c);      // a NaN norm gives NaN gradients
     }
   }
   if (h.lr_dev || h.step_dev) {

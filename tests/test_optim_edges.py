@@ -149,3 +149,25 @@ def test_moments_are_those_of_elementary_fp32_operations(where, g, seed):
             assert np.array_equal(scales.cpu().numpy(), want_scales), (name, step)
             got = codes.view(torch.uint8).cpu().numpy()
             assert np.array_equal(got, want_codes), (name, step, np.flatnonzero(got != want_codes)[:5])
+
+
+@pytest.mark.parametrize("eight", [False, True])
+@pytest.mark.parametrize("norm,grad_scale,max_norm", [(1e38, 1e3, 1.0), (3e38, -2.0 ** 20, 0.5), (1e30, 2.0 ** 60, 1e-3), (3e38, 2.0 ** -20, 1.0),
+                                                      (1e-30, 2.0 ** 100, 1.0), (1e-30, 2.0 ** -100, 1.0), (1e-30, 2.0 ** -149, 1.0),
+                                                      (2.0, 1 / 3, 0.1), (2.0, -7.0, 20.0)])
+def test_clipping_where_norm_times_grad_scale_leaves_fp32(where, norm, grad_scale, max_norm, eight):
+    """The clipped gradients have the norm that was asked for, also where norm * grad_scale or the factor alone overflow
+    or underflow."""
+    from pccl import optim
+    s = make([600], where.device, seed=72, eight=eight)
+    g = s["g"].list[0]
+    g.copy_(torch.randn(600, generator=torch.Generator().manual_seed(72)).to(where.device) * (norm / 600 ** 0.5))
+    s["g"].before = Flat.raw(s["g"].flat)
+    if not eight:
+        s["m"].list[0].zero_()
+    old = values8(s) if eight else values(s, "pgmv")
+    t = torch.tensor([norm], dtype=torch.float32, device=where.device)
+    keys = ("p", "g", "m", "r", "ms", "rs") if eight else ("p", "g", "m", "v")
+    (optim.adamw8 if eight else optim.adamw)(*(s[k].list for k in keys), 3, norm=t, max_norm=max_norm, grad_scale=grad_scale, **HYPER)
+    where.sync()
+    (check_adamw8 if eight else check_adamw)(s, old, 3, "clip", norm=float(t), max_norm=max_norm, grad_scale=grad_scale, **HYPER)
