@@ -266,7 +266,7 @@ def _plan_adamw(what, eight, params, grads, first, second, scales, copies, lr, b
                                  cptrs, n, ptypes, gtypes, ctypes_)
     else:
         native = lib.plan_adamw(ptrs(params), ptrs(grads), ptrs(first), ptrs(second), cptrs, n, ptypes, gtypes, ctypes_)
-    written = params + [c for c in copies or () if c is not None]
+    written = params + first + second + [t for s in scales or () for t in s] + [c for c in copies or () if c is not None]
     plan = AdamWPlan(lib, native, device, _hold(params, grads, first, second, copies, *(scales or ())), written)
     plan._prepare(what, grads, lr, betas, eps, weight_decay, table)
     return plan
@@ -365,9 +365,10 @@ class GradNormPlan(_Plan):
     def __call__(self, out: Optional[torch.Tensor] = None) -> torch.Tensor:
         if out is None:
             out = torch.empty(1, dtype=torch.float32, device=self._device)
+            self._run(self._norm, out.data_ptr())
         else:
-            _scalar("grad_norm", "out", out, torch.float32, self._device)
-        self._run(self._norm, out.data_ptr())
+            self._run(self._norm, _scalar("grad_norm", "out", out, torch.float32, self._device))
+            _increment_version(out)
         return out
 
 

@@ -171,3 +171,80 @@ def test_clipping_where_norm_times_grad_scale_leaves_fp32(where, norm, grad_scal
     (optim.adamw8 if eight else optim.adamw)(*(s[k].list for k in keys), 3, norm=t, max_norm=max_norm, grad_scale=grad_scale, **HYPER)
     where.sync()
     (check_adamw8 if eight else check_adamw)(s, old, 3, "clip", norm=float(t), max_norm=max_norm, grad_scale=grad_scale, **HYPER)
+
+
+# ---------------------------------------------------------------------------
+# what a call marks as modified
+# ---------------------------------------------------------------------------
+
+def test_everything_that_is_written_is_marked_as_modified(where):
+    from pccl import optim
+    n = 300
+
+    def f(x=0.0, dtype=torch.float32):
+        return torch.full((n,), x, dtype=dtype).to(where.device)
+    for eight in (False, True):
+        p, g, c, other = f(1.0), f(0.1), f(dtype=torch.bfloat16), f(0.2)
+        if eight:
+            (m, ms), (v, vs) = optim.empty_blocks(p), optim.empty_blocks(p)
+            written, lists = [p, m, v, ms, vs, c], [[p], [g], [m], [v], [ms], [vs]]
+        else:
+            m, v = f(), f()
+            written, lists = [p, m, v, c], [[p], [g], [m], [v]]
+        plan = (optim.plan_adamw8 if eight else optim.plan_adamw)(*lists, copies=[c])
+        norm = torch.ones(1).to(where.device)
+        for call in (lambda: plan(1), lambda: plan(2, grads=[other], norm=norm, max_norm=1.0),
+                     lambda: (optim.adamw8 if eight else optim.adamw)(*lists, 3, copies=[c])):
+            before, same = [t._version for t in written], [t._version for t in (g, other, norm)]
+            call()
+            assert all(t._version > b for t, b in zip(written, before)), [t._version - b for t, b in zip(written, before)]
+            assert [t._version for t in (g, other, norm)] == same
+    out, x = torch.empty(1).to(where.device), f(3.0)
+    for call in (optim.plan_grad_norm([x]), lambda o: optim.grad_norm([x], o)):
+        before = out._version, x._version
+        assert call(out) is out
+        assert out._version > before[0] and x._version == before[1]
+    codes, scales = optim.empty_blocks(x)
+    before = codes._version, scales._version, x._version
+    optim.quantize_blocks([codes], [scales], [x])
+    assert codes._version > before[0] and scales._version > before[1] and x._version == before[2]
+    before = codes._version, scales._version, x._version
+    optim.dequantize_blocks([x], [codes], [scales])
+    assert (codes._version, scales._version) == before[:2] and x._version > before[2]
+    where.sync()
+
+
+def test_a_saved_value_that_a_call_overwrites_is_noticed(where):
+    """What autograd kept of a moment, a scale or a norm raises torch's error once a call has written over it."""
+    from pccl import optim
+    p, g, m, v = (torch.full((300,), x).to(where.device) for x in (1.0, 0.1, 0.2, 0.3))
+    norm = torch.ones(1).to(where.device)
+    for saved, call in ((m, lambda: optim.adamw([p], [g], [m], [v], 1)), (v, lambda: optim.adamw([p], [g], [m], [v], 1)),
+                        (norm, lambda: optim.grad_norm([g], norm))):
+        w = torch.ones(1, requires_grad=True, device=where.device)
+        y = (w * saved).sum()
+        call()
+        with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+            y.backward()
+    where.sync()
+
+
+def test_views_and_tensors_of_inference_mode_are_written(where):
+    """Pieces of one buffer share its counter; a tensor made in inference mode has none and is written all the same."""
+    from pccl import optim
+    flat = torch.zeros(600).to(where.device)
+    m, v = torch.zeros(600).to(where.device), torch.zeros(600).to(where.device)
+    before = flat._version, m._version
+    optim.adamw([flat[:300], flat[300:]], [torch.ones(300).to(where.device)] * 2, [m[:300], m[300:]], [v[:300], v[300:]], 1)
+    where.sync()
+    assert flat._version > before[0] and m._version > before[1] and (flat != 0).all()
+    with torch.inference_mode():
+        x = torch.full((300,), 2.0).to(where.device)
+        codes, scales = optim.empty_blocks(x)
+        out = torch.empty(1).to(where.device)
+        optim.quantize_blocks([codes], [scales], [x])
+        optim.grad_norm([x], out)
+        where.sync()
+        assert (codes.float() == 448).all() and abs(float(out) - 2 * math.sqrt(300)) < 1e-4
+    optim.dequantize_blocks([x], [codes], [scales])
+    where.sync()
