@@ -248,3 +248,149 @@ def test_views_and_tensors_of_inference_mode_are_written(where):
         assert (codes.float() == 448).all() and abs(float(out) - 2 * math.sqrt(300)) < 1e-4
     optim.dequantize_blocks([x], [codes], [scales])
     where.sync()
+
+
+# ---------------------------------------------------------------------------
+# how many tensors a launch and a table hold
+# ---------------------------------------------------------------------------
+
+@pytest.mark.parametrize("count", [55, 56, 57, 63, 64, 65, 112, 113, 128, 129, 4095, 4096, 4097, 4200])
+@pytest.mark.parametrize("eight", [False, True])
+def test_exactly_so_many_tensors(where, count, eight):
+    """Tensors with elements in numbers around those that a launch (64; 56 with 8-bit moments) and a table (4096) hold, and
+    empty ones between them, which take no place: own gradients through the table, others without."""
+    from pccl import optim
+    gen = np.random.default_rng(count)
+    full = [int(x) for x in gen.choice([1, 3, 255, 256, 257, 300] if count < 1000 else [1, 2, 5, 300], count, p=None if count < 1000 else [0.5, 0.3, 0.19, 0.01])]
+    sizes = sorted(full[: count // 2]) + [0, 0, 0] + full[count // 2:] + [0]
+    keys = ("p", "g", "m", "r", "ms", "rs") if eight else ("p", "g", "m", "v")
+    s = make(sizes, where.device, g="bf16", c="f16", gap=1, seed=81, eight=eight)
+    other = make(sizes, where.device, g="bf16", gap=2, seed=82)
+    plan = (optim.plan_adamw8 if eight else optim.plan_adamw)(*(s[k].list for k in keys), copies=s["c"].list, **HYPER)
+    assert (plan._own is not None) == (count > (56 if eight else 64))
+    check, state = (check_adamw8, values8) if eight else (check_adamw, lambda s: values(s, "pgmv"))
+    old = state(s)
+    plan(3)
+    where.sync()
+    check(s, old, 3, "own gradients", **HYPER)
+    old = dict(state(s), g=values(other, "g")["g"])
+    plan(4, grads=other["g"].list)
+    where.sync()
+    check(s, old, 4, "other gradients", **HYPER)
+
+
+@pytest.mark.parametrize("counts", [[70, 70, 70], [1, 65, 3], [4100, 5, 60], [57, 0, 57]])
+@pytest.mark.parametrize("eight", [False, True])
+def test_a_table_of_several_batches(where, counts, eight):
+    """Tensors of three kinds of types, mixed: each kind has its part of the table, and one of them more than a launch serves."""
+    from pccl import optim
+    kinds = [("f32", "bf16", "bf16"), ("bf16", "bf16", None), ("f32", "f32", None)]
+    keys = ("p", "g", "m", "r", "ms", "rs") if eight else ("p", "g", "m", "v")
+    gen = np.random.default_rng(len(counts) + counts[0])
+    sets = []
+    for k, (n, (p, g, c)) in enumerate(zip(counts, kinds)):
+        sizes = [int(x) for x in gen.choice([1, 2, 5, 256, 300], n)]
+        sets.append(make(sizes, where.device, p=p, g=g, c=c, gap=1, seed=90 + k, eight=eight))
+    places = gen.permutation([(k, i) for k, n in enumerate(counts) for i in range(n)])
+    lists = [[sets[k][key].list[i] for k, i in places] for key in keys]
+    copies = [None if sets[k]["c"] is None else sets[k]["c"].list[i] for k, i in places]
+    plan = (optim.plan_adamw8 if eight else optim.plan_adamw)(*lists, copies=copies, **HYPER)
+    assert (plan._own is not None) == (max(counts) > (56 if eight else 64))
+    check, state = (check_adamw8, values8) if eight else (check_adamw, lambda s: values(s, "pgmv"))
+    for step in (3, 4):
+        old = [state(s) for s in sets]
+        plan(step)
+        where.sync()
+        for s, o in zip(sets, old):
+            check(s, o, step, f"step {step}", **HYPER)
+
+
+# ---------------------------------------------------------------------------
+# threads
+# ---------------------------------------------------------------------------
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("eight", [False, True])
+def test_a_plan_of_adamw_from_several_threads(eight):
+    """Threads on streams of their own run steps with lr, step, gradients, seed and clipping of their own, each through its
+    own plan, all at once; the results are those of the same steps one after the other."""
+    from pccl import optim
+    dev, threads, steps = "cuda:0", 4, 25
+    sizes = [300 + k for k in range(70)]
+    keys = ("p", "g", "m", "r", "ms", "rs") if eight else ("p", "g", "m", "v")
+
+    def fresh():
+        out = []
+        for k in range(threads):
+            s = make(sizes, dev, g="bf16", c="bf16", seed=100 + k, eight=eight)
+            other = make(sizes, dev, g="bf16", seed=200 + k)["g"].list
+            plan = (optim.plan_adamw8 if eight else optim.plan_adamw)(*(s[x].list for x in keys), copies=s["c"].list, **HYPER)
+            out.append((s, other, plan, torch.tensor([1.0 + k], device=dev)))
+        return out
+
+    def run(k, job):
+        s, other, plan, norm = job
+        more = dict(seed=k) if eight else {}
+        for t in range(1, steps + 1):
+            plan(t + 10 * k, lr=1e-3 * (k + 1), grad_scale=1 / (k + 1), norm=norm, max_norm=0.5 + k, grads=other if t % 3 == 0 else None, **more)
+    a, b = fresh(), fresh()
+    torch.cuda.synchronize()
+    for k in range(threads):
+        run(k, a[k])
+    errors = []
+
+    def work(k):
+        try:
+            with torch.cuda.stream(torch.cuda.Stream()):
+                run(k, b[k])
+                torch.cuda.current_stream().synchronize()
+        except BaseException as e:            # noqa: BLE001 - reported by the main thread
+            errors.append(e)
+    ts = [threading.Thread(target=work, args=(k,)) for k in range(threads)]
+    for t in ts:
+        t.start()
+    for t in ts:
+        t.join()
+    torch.cuda.synchronize()
+    assert not errors, errors
+    for k in range(threads):
+        for x in keys + ("c",):
+            assert np.array_equal(Flat.raw(a[k][0][x].flat), Flat.raw(b[k][0][x].flat)), (k, x)
+
+
+@pytest.mark.gpu
+def test_one_plan_with_other_scalars_from_several_threads():
+    """One plan, one thread after the other on streams of their own: what a call brings (lr, step, gradients) is that call's."""
+    from pccl import optim
+    dev, n = "cuda:0", 5000
+    s, t = (make([n], dev, seed=300) for _ in range(2))
+    gs = [torch.randn(n, generator=torch.Generator().manual_seed(k)).to(dev) * 0.01 for k in range(8)]
+    plan, plain = (optim.plan_adamw(*(x[k].list for k in "pgmv"), **HYPER) for x in (s, t))
+    torch.cuda.synchronize()
+    turn, errors = threading.Condition(), []
+    done = [0]
+
+    def work(k):
+        try:
+            with torch.cuda.stream(torch.cuda.Stream()):
+                with turn:
+                    turn.wait_for(lambda: done[0] == k or errors, timeout=60)
+                    plan(k + 1, lr=1e-3 * (k + 1), grads=[gs[k]])
+                    torch.cuda.current_stream().synchronize()
+                    done[0] += 1
+                    turn.notify_all()
+        except BaseException as e:            # noqa: BLE001 - reported by the main thread
+            with turn:
+                errors.append(e)
+                turn.notify_all()
+    ts = [threading.Thread(target=work, args=(k,)) for k in range(8)]
+    for x in ts:
+        x.start()
+    for x in ts:
+        x.join()
+    assert not errors, errors
+    for k in range(8):
+        plain(k + 1, lr=1e-3 * (k + 1), grads=[gs[k]])
+    torch.cuda.synchronize()
+    for key in "pmv":
+        assert np.array_equal(Flat.raw(s[key].flat), Flat.raw(t[key].flat)), key
