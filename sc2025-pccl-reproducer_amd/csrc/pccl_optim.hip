@@ -65,7 +65,8 @@ constexpr size_t kStreamFrom = (size_t)96 << 20;
 constexpr size_t kMaxItems = ((size_t)1 << 26) - 1;
 
 // Blocks of one wave: 4 KiB of what k_quantize reads (128 Mi elements, us at 1 / 2 / 4 / 8 blocks: bf16 135 101 72
-// 67), 2 KiB of what k_dequantize writes (bf16 118 82 64 66; fp32 139 107 121 122)
+// 67), 2 KiB of what k_dequantize writes (bf16 118 82 64 66; fp32 139 107 121 122).  Data that is still in the caches
+// takes the same numbers, which were not measured apart for it.
 template <class T> constexpr int kQuantizeBlocks = 4096 / (kBlock * sizeof(typename T::elem));
 template <class T> constexpr int kDequantizeBlocks = 2048 / (kBlock * sizeof(typename T::elem));
 

@@ -598,7 +598,7 @@ __host__ __device__ __forceinline__ uint32_t lead(const void* m) { return (uint3
 
 // Moments in 32 bits: one wave per 256 elements, 7-9 streams of which 4 are read
 // and 3-4 written once.  Bound by HBM: 8 x 32 Mi elements, fp32 parameters, bf16
-// gradients and copy, 7.52 GB in 1165-1180 us = 6.4-6.45 TB/s; all fp32 1145 us =
+// gradients and copy, 7.52 GB in 1161-1184 us = 6.35-6.47 TB/s; all fp32 1145 us =
 // 6.57; 300 ragged bf16 tensors, 0.94 GB in 149 us = 6.3.  Two or four times the
 // elements a wave were slower (1286, 1310 us against 1254 before the occupancy
 // was bounded, see adamw_lds): more bytes in flight spread over more DRAM pages.
@@ -638,8 +638,8 @@ __global__ __launch_bounds__(kWave) void k_adamw(AdamTable args, const void* dev
 // Moments in 8 bits: one wave per U blocks, one after the other; the loads of a
 // block are issued before the work on the one before it.  Eleven streams, and 193
 // vector instructions a block (237 with random rounding), which keep the vector
-// units about 70 % busy: 8 x 32 Mi elements, fp32 parameters, bf16 gradients and
-// copy, 4.31 GB in 692 us = 6.2 TB/s with either rounding (1, 2 or 4 blocks a
+// units 67-79 % busy: 8 x 32 Mi elements, fp32 parameters, bf16 gradients and
+// copy, 4.31 GB in 695 us = 6.2 TB/s with either rounding (1, 2 or 4 blocks a
 // wave with the best occupancy for each: 690-700).  With 16-bit parameters there
 // is less memory time to hide the start of a wave behind, and two blocks share
 // it: 2.7 GB in 512 us with one block a wave, 459 with two, 461 with four.
@@ -743,8 +743,8 @@ __global__ __launch_bounds__(kWave) void k_adamw8(Adam8Table args, const void* d
 // 8-bit blocks
 // ---------------------------------------------------------------------------
 // One wave per U blocks, whose loads are all in flight before the first is used.
-// Bound by HBM: 128 Mi elements bf16, 405 MB in 63.8 us = 6.3 TB/s; fp32, 671 MB
-// in 101 us = 6.65, with roots 102; read back to bf16 63.9 us, to fp32 107 us =
+// Bound by HBM: 128 Mi elements bf16, 405 MB in 63.7 us = 6.35 TB/s; fp32, 671 MB
+// in 101 us = 6.65, with roots 102; read back to bf16 63.5 us, to fp32 107 us =
 // 6.3 TB/s.
 template <class T, int U, bool NT>
 __global__ __launch_bounds__(kWave) void k_quantize(BlocksTable args, int count, int root) {

@@ -1,6 +1,6 @@
-"""Edges of pccl.optim: scales and codes next to a border, scalars next to the
-ends of fp32, what a call marks as modified, how many tensors a launch and a
-table hold, plans used from several threads."""
+"""Edges of pccl.optim: scalars next to the ends of fp32, the 8-bit form bit for
+bit, what a call marks as modified, how many tensors a launch and a table hold,
+plans used from several threads."""
 import math
 import threading
 
@@ -9,7 +9,7 @@ import pytest
 import torch
 
 import optim_oracle as Q
-from optim_oracle import BLOCK, TYPES, f64
+from optim_oracle import BLOCK, TYPES
 from test_optim import (HYPER, Flat, check_adamw, check_adamw8, cpu, make, values, values8, where)  # noqa: F401 - fixtures
 
 
