@@ -87,7 +87,7 @@ typedef struct {
   double lr, beta1, beta2, eps, weight_decay;   /* eps: 0, or a normal fp32 number; lr, lr weight_decay and
                                                    lr / (1 - beta1^step): finite as fp32 numbers */
   double grad_scale;        /* factor of every gradient, e.g. 1 / (loss scale * ranks); finite and not 0 as an fp32 number */
-  double max_norm;          /* clip to this norm, finite and not 0 as an fp32 number; 0 = no clipping */
+  double max_norm;          /* clip to this norm, which must not become 0 or infinite as an fp32 number; 0 = no clipping */
   int64_t step;             /* t, 1 for the first step */
   const float* lr_dev;      /* NULL, or the learning rate in device memory (replaces lr: a replayed graph reads it anew) */
   const int64_t* step_dev;  /* NULL, or t in device memory (replaces step); a value below 1 counts as 1 */

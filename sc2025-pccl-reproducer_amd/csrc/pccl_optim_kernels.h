@@ -423,7 +423,7 @@ __device__ __forceinline__ float reciprocal(float x) {
 
 // From the largest |x| of a block, as bits.  The comparison is one of integers,
 // in which NaN is above infinity, so that either becomes the scale.  The product
-// with 1 / 448 is the quotient or one unit beside it, and x * inv is within two of
+// with 1 / 448 is the quotient or one unit beside it, and x * inv within two units of
 // x / scale.  The format is defined by these products: they are what a plain form
 // in elementary operations gives on the GPU, where torch divides by a number in
 // this way, so that states agree bit for bit.  Rounded quotients were built and
